@@ -234,6 +234,61 @@ int zk_llama_decode_attn(const zk_decode_layer_t* L, const void* x, void* out, i
 int zk_llama_decode_mlp(const zk_decode_layer_t* L, const void* xa, void* out, int add_residual,
                         hipStream_t stream);
 
+/* ---- serving over a paged key / value cache -----------------------------------------------------
+ * The cache of one layer is two bf16 arrays [n_pages][page_size][Hkv * head_dim] (rotated keys, values), any
+ * page_size >= 1; row r of sequence b is row r % page_size of page page_table[b][r / page_size].
+ * Indices in device memory are checked in the kernels against the sizes given here: a slot or a page number out of
+ * range is passed over, nothing outside the arrays is touched.
+ *
+ * zk_kv_append_paged: T new tokens, packed rows q|k|v (row stride ldqkv, left untouched).  Token t is turned by row
+ * positions[t] of the cos / sin tables ([table_rows][rot_dim / 2] fp32, the values zk_rope takes) over the first
+ * rot_dim (a multiple of 16, <= head_dim) values of each q and k head: value i with i + rot_dim / 2, or, interleaved
+ * != 0, value 2i with 2i + 1; both products are rounded before the add, as in zk_rope.  The turned q goes to
+ * q_out [T][Hq * head_dim] (row stride ldq), the turned k and the v to flat cache row slots[t].  A slot outside
+ * [0, cache_rows) appends nothing; a position outside [0, table_rows) marks a padding token: its q row is zeros and
+ * nothing is appended.  Live slots of one call are distinct (of two equal ones either may win, piece by piece).
+ * (ref:inference/vlm_infer.py:259-270 decodes with use_cache=True: tf:llama:140-160 + the DynamicCache update.) */
+int zk_kv_append_paged(const void* qkv, const float* cos_t, const float* sin_t, void* q_out, void* k_cache,
+                       void* v_cache, const int32_t* positions, const int32_t* slots, int64_t T, int64_t Hq,
+                       int64_t Hkv, int64_t head_dim, int64_t rot_dim, int64_t table_rows, int64_t ldqkv, int64_t ldq,
+                       int64_t cache_rows, int interleaved, hipStream_t stream);
+
+/* zk_attn_paged: attention of the new tokens of B sequences over their cached rows (the new ones appended already).
+ * Sequence b owns rows cu_q[b] .. cu_q[b+1]-1 of q (n_b of them, 0 allowed) and ctx_lens[b] cached rows, the last
+ * n_b of which are its new tokens in order.  New token i sees every row before the new ones and, of the new ones:
+ *   tree_mask null : rows 0 .. i (a chain: single tokens, prompt chunks);
+ *   tree_mask      : row j where bit j % 64 of word tree_mask[row of q][j / 64] is set (a tree of drafted tokens;
+ *                    [T][mask_words]; bits past mask_words count as clear).
+ * out rows of tokens that see nothing are zeros; rows of q past cu_q[B] are left as they are.  Rows that a token does
+ * not see may hold anything, NaN included.  max_q >= every n_b (tokens past it are not computed) and max_ctx (an
+ * upper bound of ctx_lens that only shapes the launch) come from the host, so a captured graph serves growing caches.
+ * ws: at least what zk_attn_paged_ws says (fp32, 16-byte aligned, null when 0); calls that may overlap need one each.
+ * head_dim 64 or 128, any Hq / Hkv; softmax in fp32 (tf:llama:182-205, eager_attention_forward with a mask). */
+int zk_attn_paged(const void* q, const void* k_cache, const void* v_cache, void* out, const int32_t* page_table,
+                  const int32_t* ctx_lens, const int32_t* cu_q, const int64_t* tree_mask, float* ws, int64_t ws_floats,
+                  int64_t T, int64_t B, int64_t max_q, int64_t max_ctx, int64_t Hq, int64_t Hkv, int64_t head_dim,
+                  int64_t page_size, int64_t n_pages, int64_t table_cols, int64_t ld_table, int64_t mask_words,
+                  int64_t ldq, int64_t ldo, float scale, hipStream_t stream);
+/* workspace of such a call in floats (host arithmetic, launches nothing, needs no GPU) */
+int zk_attn_paged_ws(int64_t B, int64_t T, int64_t max_q, int64_t max_ctx, int64_t Hq, int64_t Hkv, int64_t head_dim,
+                     int64_t* ws_floats);
+
+/* ---- drawing tokens --------------------------------------------------------------------------------
+ * One token per row of bf16 logits [rows][V] (row stride ld).  Tokens stand in falling order of their logit, equal
+ * ones by the lower index; w = e^((logit - max) / temperature).  top_k > 0 keeps the first top_k; top_p < 1 the shortest
+ * prefix whose sum reaches top_p times the sum of what top_k kept; min_p > 0 those with w >= min_p; the first token is
+ * always kept.  tokens[r] = the first token whose running sum exceeds u[r] (in [0, 1)) times the kept sum;
+ * logprobs[r] = log of its share of the kept sum.  temperature 0 takes the first token.  Running sums are held in
+ * 64 bits; results do not depend on launch order.  Settings come per row (device arrays, each may be null) or for the
+ * call.  For the call: temperature in [0, 2^20], top_k >= 0, top_p in (0, 1], min_p in [0, 1], else -22.  Per row:
+ * temperature <= 0 or NaN takes the first token and values above 2^20 act as 2^20; top_k <= 0, top_p >= 1 or NaN and
+ * min_p <= 0 or NaN keep everything; top_p <= 0 or min_p > 1 keeps the first token.
+ * -inf logits are never drawn; a row of nothing else gives -1 with logprob -inf, a row with a NaN -1 with NaN.
+ * (tf generate(do_sample=True) with its logits processors; the reference itself decodes greedily, ref:vlm_infer.py:267.) */
+int zk_sample(const void* logits, const float* u, const float* temperature_rows, const int32_t* top_k_rows,
+              const float* top_p_rows, const float* min_p_rows, float temperature, int top_k, float top_p, float min_p,
+              int64_t* tokens, float* logprobs, int64_t rows, int64_t V, int64_t ld, hipStream_t stream);
+
 /* ---- LayerNorm (tf:clip:358-360,370,379,605,642; ref:adapter.py:94) ------------------
  * y = (x - mean) * rstd * gamma + beta over the last dim D (<= 8192, multiple of 8),
  * fp32 statistics.  mean/rstd [rows] fp32 are optional outputs of fwd (needed by bwd).

@@ -1,0 +1,123 @@
+"""ops.sample against a sort in 64-bit Python floats (tests/paged_ref.py), token for token."""
+import math
+import random
+
+import pytest
+import torch
+
+from tests import paged_ref as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16 = torch.bfloat16
+
+
+def f32(x):
+    return float(torch.tensor(x, dtype=torch.float32))
+
+
+def check_rows(x, u, T, k, p, mp, per_row=True, logits=None):
+    from zero_amd import ops
+    rows = x.shape[0]
+    if per_row:
+        par = dict(temperature=torch.tensor(T, device=DEV), top_k=torch.tensor(k, dtype=torch.int32, device=DEV),
+                   top_p=torch.tensor(p, device=DEV), min_p=torch.tensor(mp, device=DEV))
+    else:
+        par = dict(temperature=T[0], top_k=k[0], top_p=p[0], min_p=mp[0])
+    tok, logp = ops.sample(x.to(DEV) if logits is None else logits, torch.tensor(u, device=DEV), **par)
+    for r in range(rows):
+        i = r if per_row else 0
+        t, lp = ref.sample_row(x[r].double().tolist(), f32(u[r]), f32(T[i]), k[i], f32(p[i]), f32(mp[i]))
+        assert int(tok[r]) == t, (r, int(tok[r]), t, T[i], k[i], p[i], mp[i], u[r])
+        got = float(logp[r])
+        # a logarithm of 64-bit sums, rounded once to fp32
+        assert got == lp or (math.isnan(got) and math.isnan(lp)) or abs(got - lp) <= 2.0 ** -24 * abs(lp) + 1e-12, (got, lp)
+
+
+def settings(rng, rows):
+    return ([rng.choice([0.0, 0.2, 0.7, 1.0, 3.0]) for _ in range(rows)], [rng.choice([0, 0, 1, 2, 17, 5000]) for _ in range(rows)],
+            [rng.choice([1.0, 0.05, 0.5, 0.9, 0.999]) for _ in range(rows)], [rng.choice([0.0, 0.0, 0.01, 0.3, 1.0]) for _ in range(rows)])
+
+
+@pytest.mark.parametrize("V", [1, 2, 7, 8, 63, 1000, 1025, 9001, 32003])
+@pytest.mark.parametrize("per_row", [True, False])
+def test_sample_matches_the_sorted_row(V, per_row):
+    g, rng = torch.Generator().manual_seed(V), random.Random(V)
+    rows = 24 if V <= 9001 else 8
+    x = (torch.randn(rows, V, generator=g) * 3).to(BF16)
+    x[rows // 2:, : V // 3] = -math.inf if V > 2 else x[0, 0]
+    u = [0.0, 1 - 2.0 ** -24] + [rng.random() * (1 - 2.0 ** -23) for _ in range(rows - 2)]
+    check_rows(x, u, *settings(rng, rows), per_row=per_row)
+
+
+def test_sample_a_vocabulary_of_several_parts():
+    """More tokens than a workgroup holds at once (131 072)."""
+    g, rng = torch.Generator().manual_seed(1), random.Random(1)
+    rows, V = 6, 300007
+    x = (torch.randn(rows, V, generator=g) * 2).to(BF16)
+    x[3, :200000] = -math.inf
+    x[4] = 1.5                                                   # one value: the rank is the token
+    check_rows(x, [0.1, 0.5, 0.999, 0.3, 0.77, 0.0], [1.0, 0.5, 1.0, 2.0, 1.0, 0.0], [0, 0, 1000, 0, 0, 0],
+               [1.0, 0.9, 1.0, 0.99, 1.0, 1.0], [0.0] * 5 + [0.1])
+
+
+def test_sample_ties_go_to_the_lowest_index():
+    x = torch.tensor([[1.0, 3.0, -0.0, 3.0, 0.0, 3.0, -0.0, 1.0]] * 8).to(BF16)
+    u = [0.0, 0.3, 0.4, 0.7, 0.0, 0.999, 0.5, 0.9]
+    check_rows(x, u, [0.0, 1.0, 1.0, 1.0, 1.0, 1.0, 1.0, 50.0], [0, 1, 2, 3, 4, 8, 0, 0], [1.0] * 6 + [0.34, 1.0], [0.0] * 8)
+    y = torch.zeros(4, 70000).to(BF16)                            # more equal tokens than 16 bits count
+    y[1, ::2] = -0.0
+    y[2, 5] = 1e-30
+    check_rows(y, [0.0, 0.9999, 0.5, 0.25], [1.0] * 4, [0, 0, 0, 33], [1.0, 1.0, 0.5, 1.0], [0.0] * 4)
+
+
+def test_sample_extreme_rows():
+    """Rows without a token, with NaN, infinities, the type's lowest value as a mask, values of far magnitudes."""
+    low, big = torch.finfo(BF16).min, torch.finfo(BF16).max
+    base = (torch.randn(12, 64, generator=torch.Generator().manual_seed(3)) * 2)
+    base[0] = -math.inf
+    base[1, 5] = math.nan
+    base[2, 9] = -math.nan
+    base[3, 7], base[3, 9] = math.inf, math.inf
+    base[4, 8:] = low
+    base[5] = low
+    base[6, 1], base[6, 2] = big, low
+    base[7] = torch.tensor([(-1.0) ** i * 2.0 ** (i - 60) for i in range(64)])
+    base[8] = -torch.tensor([2.0 ** (i - 30) for i in range(64)])
+    base[9, 1:] = -math.inf
+    base[10] = math.inf
+    x = base.to(BF16)
+    for u in (0.0, 0.31, 0.97):
+        check_rows(x, [u] * 12, [1.0] * 12, [0] * 12, [1.0] * 12, [0.0] * 12)
+        check_rows(x, [u] * 12, [1e9] * 12, [0, 3] * 6, [0.8] * 12, [0.0] * 12)
+        check_rows(x, [u] * 12, [0.0] * 12, [0] * 12, [1.0] * 12, [0.0] * 12)
+
+
+def test_sample_settings_out_of_their_ranges_per_row():
+    x = (torch.randn(10, 200, generator=torch.Generator().manual_seed(5)) * 2).to(BF16)
+    nan = math.nan
+    check_rows(x, [0.6] * 8 + [-1.0, 2.0], [-1.0, nan, 1.0, 1.0, 1.0, 1.0, 1.0, 1.0, 1.0, 1.0],
+               [0, 0, -3, 0, 0, 0, 0, 0, 0, 0], [1.0, 1.0, 1.0, -0.5, 0.0, 7.0, nan, 1.0, 1.0, 1.0],
+               [0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 5.0, nan, -1.0])
+
+
+def test_sample_strided_rows_and_every_alignment():
+    g = torch.Generator().manual_seed(6)
+    wide = (torch.randn(9, 1200, generator=g) * 2).to(BF16)
+    dev = wide.to(DEV)
+    for start, V in ((0, 1000), (1, 999), (3, 513), (8, 800), (5, 1)):
+        check_rows(wide[:, start:start + V], [0.05 + 0.1 * i for i in range(9)], [1.0] * 9, [0] * 9, [0.95] * 9, [0.0] * 9,
+                   logits=dev[:, start:start + V])
+
+
+def test_sample_follows_the_distribution():
+    """A row's tokens over many u: shares within 5 standard deviations of their probability."""
+    from zero_amd import ops
+    x = torch.tensor([0.0, 1.0, 2.0, -1.0, 0.5], dtype=BF16)
+    n = 40000
+    u = (torch.arange(n, dtype=torch.float64) + 0.5) / n          # evenly spread: every share is exact to a step
+    tok, logp = ops.sample(x.expand(n, 5).contiguous().to(DEV), u.float().to(DEV), temperature=0.7)
+    p = torch.softmax(x.double() / f32(0.7), 0)
+    share = torch.bincount(tok.cpu(), minlength=5).double() / n
+    assert ((share - p).abs() <= 2.0 / n).all()
+    assert torch.allclose(logp.cpu().double(), p.log()[tok.cpu()], rtol=1e-6, atol=1e-7)

@@ -40,6 +40,10 @@ SIGNATURES = {
     "zk_attn_decode_fused_static": [_P, _P, _P, _P, _P, _P, _L, _L, _L, _L, _L, _L, _L, _L, _F, _P],
     "zk_llama_decode_attn": [_P, _P, _P, _I, _P],
     "zk_llama_decode_mlp": [_P, _P, _P, _I, _P],
+    "zk_kv_append_paged": [_P, _P, _P, _P, _P, _P, _P, _P, _L, _L, _L, _L, _L, _L, _L, _L, _L, _I, _P],
+    "zk_attn_paged": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _L, _L, _L, _L, _L, _L, _L, _L, _L, _L, _L, _L, _L, _L, _L, _F, _P],
+    "zk_attn_paged_ws": [_L, _L, _L, _L, _L, _L, _L, _P],
+    "zk_sample": [_P, _P, _P, _P, _P, _P, _F, _I, _F, _F, _P, _P, _L, _L, _L, _P],
     "zk_layernorm_fwd": [_P, _P, _P, _P, _P, _P, _L, _L, _F, _P],
     "zk_layernorm_bwd": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _L, _L, _L, _P],
     "zk_rmsnorm_fwd": [_P, _P, _P, _P, _L, _L, _F, _P],

@@ -282,6 +282,154 @@ def attn_decode_fused(qkv, cos_t, sin_t, k_cache, v_cache, pos: int, Hq: int, Hk
     return out
 
 
+def _here(name: str, *tensors):
+    """The call's tensors are on the current device, where the kernel is launched (None passes)."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name}: zero_amd kernels need ROCm device tensors (no CPU path exists)")
+        if dev is None:
+            dev = torch.cuda.current_device()
+        if t.get_device() != dev:
+            raise ValueError(f"{name}: a tensor on cuda:{t.get_device()}, but the current device is cuda:{dev}")
+
+
+def _chk_paged_cache(name: str, k_cache, v_cache, width: int):
+    for t in (k_cache, v_cache):
+        if t.dtype != BF16 or t.dim() != 3 or t.shape[2] != width or not t.is_contiguous():
+            raise ValueError(f"{name}: caches must be contiguous bf16 [pages, page_size, Hkv*hd]")
+    if k_cache.shape != v_cache.shape:
+        raise ValueError(f"{name}: key and value caches differ in shape")
+
+
+def _chk_i32(name: str, t, n: int, what: str):
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name}: {what} must be contiguous int32 [{n}]")
+
+
+def kv_append_paged(qkv, cos_t, sin_t, k_cache, v_cache, positions, slots, Hq: int, Hkv: int, hd: int,
+                    interleaved: bool = False, q_out=None):
+    """T new tokens into a paged cache: rotated keys and values go to the flat cache rows ``slots`` (int32 [T]; outside
+    the cache, e.g. -1: nothing is appended), the rotated queries are returned [T, Hq*hd].
+    qkv: [T, (Hq + 2 Hkv) * hd] packed, before the rotation (left untouched); cos_t / sin_t fp32 [P, rot/2], rot <= hd a
+    multiple of 16: the first rot values of a head turn by row ``positions[t]`` (int32 [T]; outside the table: a padding
+    token, q row of zeros and nothing appended), value i with i + rot/2, or 2i with 2i + 1 (``interleaved``).
+    Caches: contiguous [pages, page_size, Hkv*hd]; the live slots of one call are distinct."""
+    name = "kv_append_paged"
+    _here(name, qkv, cos_t, sin_t, k_cache, v_cache, positions, slots, q_out)
+    _chk2d(qkv, "qkv")
+    T = qkv.shape[0]
+    if Hq <= 0 or Hkv <= 0 or Hq % Hkv or qkv.shape[1] != (Hq + 2 * Hkv) * hd:
+        raise ValueError(f"{name}: qkv must be [T, (Hq + 2 Hkv) * hd]")
+    _chk_paged_cache(name, k_cache, v_cache, Hkv * hd)
+    if (cos_t.dtype != torch.float32 or cos_t.dim() != 2 or not cos_t.is_contiguous() or sin_t.dtype != torch.float32
+            or sin_t.shape != cos_t.shape or not sin_t.is_contiguous()):
+        raise ValueError(f"{name}: cos / sin tables must be contiguous fp32 [positions, rot / 2]")
+    _chk_i32(name, positions, T, "positions"); _chk_i32(name, slots, T, "slots")
+    if q_out is None:
+        q_out = torch.empty((T, Hq * hd), dtype=BF16, device=qkv.device)
+    else:
+        _chk2d(q_out, "q_out")
+        if q_out.shape != (T, Hq * hd):
+            raise ValueError(f"{name}: q_out must be [T, Hq * hd]")
+    if T == 0:
+        return q_out
+    rows, half = cos_t.shape
+    check(lib.zk_kv_append_paged(qkv.data_ptr(), cos_t.data_ptr(), sin_t.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(),
+                                 v_cache.data_ptr(), positions.data_ptr(), slots.data_ptr(), T, Hq, Hkv, hd, 2 * half, rows,
+                                 _ld(qkv), _ld(q_out), k_cache.shape[0] * k_cache.shape[1], int(interleaved), _stream()),
+          "zk_kv_append_paged")
+    return q_out
+
+
+def attn_paged_ws_floats(B: int, T: int, max_q: int, max_ctx: int, Hq: int, Hkv: int, hd: int) -> int:
+    """fp32 values of workspace that attn_paged needs for such a call."""
+    n = ctypes.c_int64()
+    check(lib.zk_attn_paged_ws(B, T, max_q, max_ctx, Hq, Hkv, hd, ctypes.addressof(n)), "zk_attn_paged_ws")
+    return n.value
+
+
+def attn_paged(q, k_cache, v_cache, page_table, ctx_lens, cu_q, max_q: int, max_ctx: int, Hq: int, Hkv: int, hd: int,
+               scale: float, tree_mask=None, out=None, ws=None):
+    """Attention of the new tokens of B sequences over a paged cache that holds them already.  q [T, Hq*hd]: rows
+    cu_q[b] .. cu_q[b+1]-1 (int32 [B+1]) are the n_b new tokens of sequence b, the last n_b of its ctx_lens[b]
+    (int32 [B]) cached rows; row r is row r % page_size of page page_table[b, r // page_size] (int32 [B, cols]).
+    A new token sees all rows before the new ones and, of those, the ones up to its own (tree_mask None) or the ones its
+    bits name (tree_mask int64 [T, words], bit j % 64 of word j // 64 = new token j of the sequence; see
+    inference.paged.tree_mask).  A token that sees nothing gets zeros.  max_q >= every n_b; max_ctx: an upper bound of
+    ctx_lens that only shapes the launch.  Rows of q past cu_q[B] are left as they are in ``out``.
+    ws: fp32 workspace of at least attn_paged_ws_floats(...) values (allocated when not given)."""
+    name = "attn_paged"
+    _here(name, q, k_cache, v_cache, page_table, ctx_lens, cu_q, tree_mask, out, ws)
+    _chk2d(q, "q")
+    T = q.shape[0]
+    if Hq <= 0 or Hkv <= 0 or Hq % Hkv or q.shape[1] != Hq * hd:
+        raise ValueError(f"{name}: q must be [T, Hq * hd] with Hq a multiple of Hkv")
+    _chk_paged_cache(name, k_cache, v_cache, Hkv * hd)
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1:
+        raise ValueError(f"{name}: page_table must be int32 [B, columns]")
+    B, cols = page_table.shape
+    _chk_i32(name, ctx_lens, B, "ctx_lens"); _chk_i32(name, cu_q, B + 1, "cu_q")
+    words = 0
+    if tree_mask is not None:
+        if tree_mask.dtype != torch.int64 or tree_mask.dim() != 2 or tree_mask.shape[0] != T or not tree_mask.is_contiguous():
+            raise ValueError(f"{name}: tree_mask must be contiguous int64 [T, words]")
+        words = tree_mask.shape[1]
+    if out is None:
+        out = torch.empty((T, Hq * hd), dtype=BF16, device=q.device)
+    else:
+        _chk2d(out, "out")
+        if out.shape != (T, Hq * hd):
+            raise ValueError(f"{name}: out must be [T, Hq * hd]")
+    need = attn_paged_ws_floats(B, T, max_q, max_ctx, Hq, Hkv, hd)
+    if ws is None:
+        if need:
+            ws = torch.empty(need, dtype=torch.float32, device=q.device)
+    elif ws.dtype != torch.float32 or not ws.is_contiguous() or ws.numel() < need:
+        raise ValueError(f"{name}: ws must be contiguous fp32 with at least {need} values")
+    if T == 0:
+        return out
+    check(lib.zk_attn_paged(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), page_table.data_ptr(),
+                            ctx_lens.data_ptr(), cu_q.data_ptr(), _p(tree_mask), _p(ws), ws.numel() if ws is not None else 0,
+                            T, B, max_q, max_ctx, Hq, Hkv, hd, k_cache.shape[1], k_cache.shape[0], cols, _ld(page_table),
+                            words, _ld(q), _ld(out), scale, _stream()), "zk_attn_paged")
+    return out
+
+
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Draws a token per row of bf16 logits [rows, V] with the numbers u (fp32 [rows], in [0, 1)); returns (tokens int64
+    [rows], log-probabilities fp32 [rows] of the drawn tokens among the kept ones).  Settings are numbers for the call or
+    tensors [rows] (fp32; top_k int32): temperature 0 = the largest logit; top_k 0, top_p 1 and min_p 0 keep everything.
+    Tokens stand in falling order of their logit, equal ones by the lower index: top_k keeps the first, top_p the shortest
+    prefix that reaches its share of what top_k kept, min_p those with at least that share of the largest's probability;
+    the token drawn is the first whose running sum exceeds u times the kept sum (64-bit sums).  -inf is never drawn; a row
+    of -inf gives token -1 with -inf, a row with a NaN -1 with NaN."""
+    name = "sample"
+    rows_of = [v if torch.is_tensor(v) else None for v in (temperature, top_k, top_p, min_p)]
+    _here(name, logits, u, *rows_of)
+    _chk2d(logits, "logits")
+    rows, V = logits.shape
+    if V == 0:
+        raise ValueError(f"{name}: empty vocabulary")
+    for t, n, d in zip([u] + rows_of, ("u", "temperature", "top_k", "top_p", "min_p"),
+                       (torch.float32, torch.float32, torch.int32, torch.float32, torch.float32)):
+        if t is not None and (t.dtype != d or t.dim() != 1 or t.shape[0] != rows or (rows > 1 and t.stride(0) != 1)):
+            raise ValueError(f"{name}: {n} must be a contiguous {d} tensor [{rows}]")
+    t, k, p, mp = (0 if r is not None else v for r, v in zip(rows_of, (temperature, top_k, top_p, min_p)))
+    if ((rows_of[0] is None and not 0 <= t <= 2 ** 20) or (rows_of[1] is None and not (0 <= k < 2 ** 31 and k == int(k)))
+            or (rows_of[2] is None and not 0 < p <= 1) or (rows_of[3] is None and not 0 <= mp <= 1)):
+        raise ValueError(f"{name}: temperature in [0, 2^20], top_k a whole number >= 0, top_p in (0, 1], min_p in [0, 1]")
+    tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    logp = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    if rows == 0:
+        return tokens, logp
+    check(lib.zk_sample(logits.data_ptr(), u.data_ptr(), _p(rows_of[0]), _p(rows_of[1]), _p(rows_of[2]), _p(rows_of[3]),
+                        t, int(k), p, mp, tokens.data_ptr(), logp.data_ptr(), rows, V, _ld(logits), _stream()), "zk_sample")
+    return tokens, logp
+
+
 def layernorm_fwd(x, gamma, beta, eps: float, save_stats: bool = True):
     _chk2d(x, "x"); _chk_flat(gamma, "gamma"); _chk_flat(beta, "beta")
     if not x.is_contiguous():
