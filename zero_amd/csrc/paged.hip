@@ -88,83 +88,352 @@ struct PagedArgs {
   bf16_t* out;
   const int *table, *ctx, *cu;
   const unsigned long long* mask;
+  float *part_o, *part_ml;      // [T * Hq][splits][HD] un-normalised outputs, [..][2] maximum and sum; null: one split
   int T, B, Hq, Hkv, page_size, n_pages, table_cols, ld_table, mask_words;
+  int tiles, splits, split_keys;
   long long ldq, ldo;
   float scale;
 };
 
+// one sequence's share of the call
+struct Seq {
+  int q0, n, len;               // first row of q, new tokens, cached rows
+  long long first;              // cached rows before the new tokens (as the lengths say: negative if they do not fit)
+  __device__ __forceinline__ Seq(const PagedArgs& a, int b) {
+    q0 = min(max(a.cu[b], 0), a.T);
+    n = min(max(a.cu[b + 1], q0), a.T) - q0;
+    len = (int)min((long long)max(a.ctx[b], 0), (long long)a.table_cols * a.page_size);
+    first = (long long)a.ctx[b] - n;
+  }
+};
+
+// which of the 32 keys from `base` on new token i (row q0 + i of q) may see, as bits; the cache's end is not looked at
+__device__ __forceinline__ unsigned seen_bits(const PagedArgs& a, const Seq& s, int i, long long base) {
+  const long long j0 = base - s.first;              // key `base` is new token j0 (negative: a row before them)
+  if (j0 + 32 <= 0) return ~0u;
+  if (!a.mask) {                                    // keys up to the token's own
+    const long long c = i - j0 + 1;
+    return c >= 32 ? ~0u : c <= 0 ? 0u : (1u << (int)c) - 1u;
+  }
+  const unsigned long long* m = a.mask + (size_t)(s.q0 + i) * a.mask_words;
+  if (j0 < 0) return (unsigned)(m[0] << (int)-j0) | ((1u << (int)-j0) - 1u);
+  const long long w = j0 >> 6;
+  const int sh = (int)(j0 & 63);
+  unsigned long long x = w < a.mask_words ? m[w] >> sh : 0ull;
+  if (sh > 32 && w + 1 < a.mask_words) x |= m[w + 1] << (64 - sh);
+  return (unsigned)x;
+}
+
+// flat cache row of key `key` of sequence b, or -1: past `end`, or on a page that does not exist
+__device__ __forceinline__ int cache_row(const PagedArgs& a, int b, int key, int end) {
+  if (key >= end) return -1;
+  const unsigned pg = (unsigned)a.table[(size_t)b * a.ld_table + (unsigned)key / (unsigned)a.page_size];
+  return pg < (unsigned)a.n_pages ? (int)(pg * (unsigned)a.page_size + (unsigned)key % (unsigned)a.page_size) : -1;
+}
+
+__device__ __forceinline__ bool not_finite(unsigned w) {
+  return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
+}
+
 // =========================================================================================
-// attention, one wave per (new token, query head): 64 keys at a time, a lane scores one key, then owns hd / 64 output
-// columns.  Running maximum and sum of the softmax in fp32.
+// attention.  The q rows of a group of Hq / Hkv heads read the same keys, so a tile is 16 * MT rows (token i, head g of the
+// group at row i * G + g) of one kv head, and a workgroup is (sequence, kv head, row tile, share of the keys).
+// Four waves take 32-key pieces in turn, each with a softmax of its own (running maximum and sum in fp32, no barrier in
+// the loop), merged through LDS at the end; shares of one sequence are merged by attn_paged_merge_kernel.
+// Products: 16x16x32 MFMAs.  S^T[key][row] = K Q^T, K fragments straight from memory to registers (16 rows x 64 bytes per
+// load); a lane then owns 8 keys of one row, which are the B operand of O^T += V^T P^T as they stand if V^T is read in
+// the same key order (elements 0-3 keys 4g.., 4-7 keys 16 + 4g.. of lane group g): ds_read_b64_tr_b16 from the wave's own
+// copy of V in LDS, chunk-swizzled by the row.  The next piece's rows are requested as soon as a piece's registers are free.
 // =========================================================================================
 template <int HD>
-__global__ __launch_bounds__(64) void attn_paged_rows_kernel(PagedArgs a) {
-  constexpr int CPL = HD / 64;
-  __shared__ float qs[HD];
-  __shared__ float ps[64];
-  __shared__ long long rows[64];
-  const int lane = threadIdx.x, t = blockIdx.x / a.Hq, h = blockIdx.x % a.Hq, kvh = h / (a.Hq / a.Hkv);
+struct Merge {
+  static constexpr int LDO = HD + 4;                // floats per row of the waves' exchange: 16 rows hit different banks
+};
+
+template <int HD, int MT>
+__global__ __launch_bounds__(256, MT == 1 ? (HD == 128 ? 3 : 4) : MT == 2 ? 2 : 1) void attn_paged_stream_kernel(PagedArgs a) {
+  constexpr int CPR = HD / 8, KC = HD / 32, DB = HD / 16, NV = HD / 16, LDO = Merge<HD>::LDO;
+  constexpr int VB = 32 * HD * 2;                   // one wave's V piece
+  constexpr int XB = 4 * 16 * LDO * 4;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[XB > 4 * VB ? XB : 4 * VB];
+  __shared__ float sm[4][16 * MT], sl[4][16 * MT];
+  const int tid = threadIdx.x, lane = tid & 63, g4 = lane >> 4, col = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int id = blockIdx.x;
+  const int kvh = id % a.Hkv; id /= a.Hkv;
+  const int tile = id % a.tiles; id /= a.tiles;
+  const int split = id % a.splits;
+  const int b = id / a.splits;
+  const Seq s(a, b);
+  const int G = a.Hq / a.Hkv, rows = s.n * G, r0 = tile * 16 * MT, kvw = a.Hkv * HD;
+  const int ks = split * a.split_keys;
+  if (r0 >= rows || (split > 0 && ks >= s.len)) return;
+  const int ke = split == a.splits - 1 ? s.len : min(s.len, ks + a.split_keys);
+  const bool alone = ks == 0 && ke == s.len;        // no other share of this sequence
+  const float sc = a.scale * kLog2e;
+  const bf16_t* kb = a.k + kvh * HD;
+  const bf16_t* vb = a.v + kvh * HD;
+
+  bf16x8 q[MT][KC];
+  int tok[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int r = r0 + mt * 16 + col;
+    tok[mt] = min(r, rows - 1) / G;
+    const bf16_t* qp = a.q + (size_t)(s.q0 + tok[mt]) * a.ldq + (size_t)(kvh * G + min(r, rows - 1) % G) * HD + 8 * g4;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) q[mt][c] = *reinterpret_cast<const bf16x8*>(qp + 32 * c);
+  }
+  f32x4 o[MT][DB];
+  float m[MT], l[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    m[mt] = -INFINITY; l[mt] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[mt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  unsigned char* vl = smem + wave * VB;
+  bf16x8 kf[2][KC];
+  u32x4 vr[NV];
+  f32x4 sc4[MT][2];
+  bf16x8 p[MT];
+  auto request = [&](int r) __attribute__((always_inline)) {      // a piece's rows; lane & 31 holds key lane & 31's
+#pragma unroll
+    for (int kg = 0; kg < 2; ++kg) {
+      const bf16_t* x = kb + (size_t)max(__shfl(r, kg * 16 + col, 64), 0) * kvw + 8 * g4;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) kf[kg][c] = *reinterpret_cast<const bf16x8*>(x + 32 * c);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int idx = i * 64 + lane;
+      vr[i] = *reinterpret_cast<const u32x4*>(vb + (size_t)max(__shfl(r, idx / CPR, 64), 0) * kvw + (idx % CPR) * 8);
+    }
+  };
+  auto scores = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int kg = 0; kg < 2; ++kg)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        f32x4 z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < KC; ++c) z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[kg][c], q[mt][c], z, 0, 0, 0);
+        sc4[mt][kg] = z;
+      }
+  };
+  auto v_at = [&](int vrow, int ch) { return vl + vrow * (HD * 2) + ((ch ^ ((vrow & (CPR / 2 - 1)) << 1)) << 4); };
+  // a value's lanes write, other lanes read: nothing may move across in the compiler either (the wave's own LDS
+  // instructions are in order)
+  auto lds_turn = [&]() __attribute__((always_inline)) {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+  };
+  auto softmax = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      float mx = sc4[mt][0][0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) mx = fmaxf(mx, sc4[mt][e >> 2][e & 3]);
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float mn = fmaxf(m[mt], mx * sc);
+      const float use = mn == -INFINITY ? 0.f : mn;
+      const float f = __builtin_amdgcn_exp2f(m[mt] - use);
+      l[mt] *= f;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[mt][d] *= f;
+      m[mt] = mn;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc4[mt][e >> 2][e & 3], sc, -use));
+        l[mt] += x;
+        p[mt][e] = (__bf16)x;                       // rounded to bf16 for the matrix product only
+      }
+    }
+  };
+  auto product = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      const unsigned char* at = v_at(4 * g4 + (col >> 2), 2 * d + ((col & 3) >> 1)) + (col & 1) * 8;
+      union { struct { short4_t lo, hi; } h; bf16x8 v; } u;
+      u.h.lo = lds_read_tr16(at);
+      u.h.hi = lds_read_tr16(at + 16 * (HD * 2));   // 16 rows on: the same swizzle
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) o[mt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u.v, p[mt], o[mt][d], 0, 0, 0);
+    }
+  };
+
+  // pieces that every row of the tile sees whole: up to the tile's first token in a chain, to the new tokens in a tree
+  const long long clear = s.first + (a.mask ? 0 : r0 / G + 1);
+  const int bulk = (int)min((long long)ke, max(clear, 0ll));
+  int base = ks + 32 * wave;
+  if (base + 32 <= bulk) {
+    int row = cache_row(a, b, base + (lane & 31), bulk);
+    request(row);
+    int ahead = cache_row(a, b, base + 128 + (lane & 31), bulk);
+    while (__all(row >= 0)) {
+      scores();
+#pragma unroll
+      for (int i = 0; i < NV; ++i) *reinterpret_cast<u32x4*>(v_at((i * 64 + lane) / CPR, (i * 64 + lane) % CPR)) = vr[i];
+      lds_turn();
+      base += 128;
+      row = ahead;
+      if (base + 32 <= bulk) {
+        request(row);
+        ahead = cache_row(a, b, base + 128 + (lane & 31), bulk);
+      }
+      softmax();
+      product();
+      lds_turn();
+      if (base + 32 > bulk) break;
+    }
+  }
+  // the others: the cache's end, new tokens, pages that do not exist (and what stands behind one)
+  for (; base < ke; base += 128) {
+    const int row = cache_row(a, b, base + (lane & 31), ke);
+    request(row);
+    scores();
+    const unsigned ok = (unsigned)__ballot(row >= 0);
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int vrow = (i * 64 + lane) / CPR;
+      u32x4 x = vr[i];
+      if (!((ok >> vrow) & 1)) x = u32x4{0u, 0u, 0u, 0u};      // its p is 0, and 0 x NaN is not
+#pragma unroll
+      for (int e = 0; e < 4; ++e) odd |= not_finite(x[e]);
+      *reinterpret_cast<u32x4*>(v_at(vrow, (i * 64 + lane) % CPR)) = x;
+    }
+    lds_turn();
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const unsigned vis = seen_bits(a, s, tok[mt], base) & ok;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (!((vis >> (16 * (e >> 2) + 4 * g4 + (e & 3))) & 1)) sc4[mt][e >> 2][e & 3] = -INFINITY;
+    }
+    softmax();
+    if (!__any(odd)) {
+      product();
+    } else {
+      // infinities or NaN among rows that some of the tile may not see: key by key, rows with p = 0 passed over
+#pragma unroll 1
+      for (int vrow = 0; vrow < 32; ++vrow) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          float x = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e == 4 * (vrow >> 4) + (vrow & 3)) x = (float)p[mt][e];
+          x = __shfl(x, ((vrow >> 2) & 3) * 16 + col, 64);
+          if (x == 0.f) continue;
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
+            const u32x2 w = *reinterpret_cast<const u32x2*>(v_at(vrow, 2 * d + (g4 >> 1)) + (g4 & 1) * 8);
+            o[mt][d][0] += x * lo_bf(w[0]); o[mt][d][1] += x * hi_bf(w[0]);
+            o[mt][d][2] += x * lo_bf(w[1]); o[mt][d][3] += x * hi_bf(w[1]);
+          }
+        }
+      }
+    }
+    lds_turn();
+  }
+  // ---- the four waves' shares, in wave order
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    l[mt] += __shfl_xor(l[mt], 16, 64);
+    l[mt] += __shfl_xor(l[mt], 32, 64);
+    if (g4 == 0) { sm[wave][mt * 16 + col] = m[mt]; sl[wave][mt * 16 + col] = l[mt]; }
+  }
+  float* xo = reinterpret_cast<float*>(smem);
+  const int per = HD / 16, orow = tid >> 4, oc = (tid & 15) * per;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    __syncthreads();
+    {
+      const int r = mt * 16 + col;
+      const float M = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
+      const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[mt] - M);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4*>(xo + (wave * 16 + col) * LDO + d * 16 + 4 * g4) = o[mt][d] * f;
+    }
+    __syncthreads();
+    const int r = r0 + mt * 16 + orow;
+    if (r < rows) {
+      const int lr = mt * 16 + orow;
+      const float M = fmaxf(fmaxf(sm[0][lr], sm[1][lr]), fmaxf(sm[2][lr], sm[3][lr]));
+      float L = 0.f, y[per];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) L += M == -INFINITY ? 0.f : sl[w][lr] * __builtin_amdgcn_exp2f(sm[w][lr] - M);
+#pragma unroll
+      for (int e = 0; e < per; ++e)
+        y[e] = (xo[orow * LDO + oc + e] + xo[(16 + orow) * LDO + oc + e]) +
+               (xo[(32 + orow) * LDO + oc + e] + xo[(48 + orow) * LDO + oc + e]);
+      const int t = s.q0 + r / G, h = kvh * G + r % G;
+      if (alone) {
+        const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);      // nothing seen: zeros; NaN stays NaN
+        bf16_t* op = a.out + (size_t)t * a.ldo + (size_t)h * HD + oc;
+#pragma unroll
+        for (int e = 0; e < per; e += 4) {
+          u32x2 w = {pack2bf(y[e] * inv, y[e + 1] * inv), pack2bf(y[e + 2] * inv, y[e + 3] * inv)};
+          *reinterpret_cast<u32x2*>(op + e) = w;
+        }
+      } else {
+        const size_t part = ((size_t)t * a.Hq + h) * a.splits + split;
+#pragma unroll
+        for (int e = 0; e < per; e += 4)
+          *reinterpret_cast<f32x4*>(a.part_o + part * HD + oc + e) = f32x4{y[e], y[e + 1], y[e + 2], y[e + 3]};
+        if (oc == 0) { a.part_ml[part * 2] = M; a.part_ml[part * 2 + 1] = L; }
+      }
+    }
+  }
+}
+
+// out = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the shares of a row's sequence, in order: one workgroup of
+// HD threads per (token, head)
+template <int HD>
+__global__ __launch_bounds__(HD) void attn_paged_merge_kernel(PagedArgs a) {
+  const int t = blockIdx.x / a.Hq, h = blockIdx.x % a.Hq, d = threadIdx.x;
   int lo = 0, hi = a.B;                             // last sequence that starts at or before row t
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (a.cu[mid] <= t) lo = mid; else hi = mid;
   }
-  const int b = lo, q0 = a.cu[b], q1 = a.cu[b + 1];
-  if (t < q0 || t >= q1) return;                    // rows behind the last sequence stay as they are
-  const int len = min(max(a.ctx[b], 0), (int)min((long long)a.table_cols * a.page_size, 0x7FFFFFFFLL));
-  const long long first = (long long)a.ctx[b] - (q1 - q0);
-  const int kvw = a.Hkv * HD, i = t - q0;
-  for (int d = lane; d < HD; d += 64) qs[d] = bf2f(a.q[(size_t)t * a.ldq + h * HD + d]) * (a.scale * kLog2e);
-  __syncthreads();
-  float m = -INFINITY, l = 0.f, acc[CPL];
-#pragma unroll
-  for (int c = 0; c < CPL; ++c) acc[c] = 0.f;
-  for (int k0 = 0; k0 < len; k0 += 64) {
-    const int key = k0 + lane;
-    bool seen = key < len;
-    const long long j = (long long)key - first;     // which new token this row is (negative: a row before them)
-    if (seen && j >= 0) {
-      if (a.mask) seen = (j >> 6) < a.mask_words && ((a.mask[(size_t)t * a.mask_words + (j >> 6)] >> (j & 63)) & 1);
-      else seen = j <= i;
-    }
-    long long r = -1;
-    if (seen) {
-      const int pg = a.table[(size_t)b * a.ld_table + key / a.page_size];
-      if (pg >= 0 && pg < a.n_pages) r = (long long)pg * a.page_size + key % a.page_size;
-    }
-    float s = -INFINITY;
-    if (r >= 0) {
-      const bf16_t* kp = a.k + (size_t)r * kvw + kvh * HD;
-      s = 0.f;
-      for (int c = 0; c < HD / 8; ++c) {
-        const u32x4 kr = *reinterpret_cast<const u32x4*>(kp + c * 8);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s += lo_bf(kr[e]) * qs[c * 8 + 2 * e] + hi_bf(kr[e]) * qs[c * 8 + 2 * e + 1];
-      }
-    }
-    const float mn = fmaxf(m, wave_max(s));
-    const float base = mn == -INFINITY ? 0.f : mn;
-    const float p = r >= 0 ? __builtin_amdgcn_exp2f(s - base) : 0.f;
-    const float f = __builtin_amdgcn_exp2f(m - base);
-    __syncthreads();
-    ps[lane] = p;
-    rows[lane] = r;
-    __syncthreads();
-    l = l * f + wave_sum(p);
-    m = mn;
-#pragma unroll
-    for (int c = 0; c < CPL; ++c) acc[c] *= f;
-    for (int kk = 0; kk < 64; ++kk) {
-      const long long rr = rows[kk];
-      if (rr < 0) continue;
-      const bf16_t* vp = a.v + (size_t)rr * kvw + kvh * HD + lane * CPL;
-#pragma unroll
-      for (int c = 0; c < CPL; ++c) acc[c] += ps[kk] * bf2f(vp[c]);
-    }
+  const Seq s(a, lo);
+  if (t < s.q0 || t >= s.q0 + s.n) return;
+  const int parts = min(a.splits, (s.len + a.split_keys - 1) / a.split_keys);
+  if (parts <= 1) return;                           // written by its only share
+  const size_t p0 = (size_t)blockIdx.x * a.splits;
+  float M = -INFINITY;
+  for (int i = 0; i < parts; ++i) M = fmaxf(M, a.part_ml[(p0 + i) * 2]);
+  float L = 0.f, y = 0.f;
+  for (int i = 0; i < parts; ++i) {
+    const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(a.part_ml[(p0 + i) * 2] - M);
+    L += a.part_ml[(p0 + i) * 2 + 1] * f;
+    y += a.part_o[(p0 + i) * HD + d] * f;
   }
-  const float inv = l > 0.f ? 1.0f / l : 0.f;       // a row that sees nothing is zero
-#pragma unroll
-  for (int c = 0; c < CPL; ++c) a.out[(size_t)t * a.ldo + h * HD + lane * CPL + c] = f2bf(acc[c] * inv);
+  const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
+  a.out[(size_t)t * a.ldo + (size_t)h * HD + d] = f2bf(y * inv);
+}
+
+// shape of a launch: host arithmetic on the sizes alone
+struct Plan {
+  int mt, tiles, splits, split_keys;
+};
+inline Plan plan_of(int64_t B, int64_t max_q, int64_t max_ctx, int64_t Hq, int64_t Hkv) {
+  Plan p;
+  const int64_t rows = max_q * (Hq / Hkv);
+  p.mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  p.tiles = (int)((rows + 16 * p.mt - 1) / (16 * p.mt));
+  // shares of the keys: enough workgroups for four rounds of the 256 CUs, none under 128 keys (one piece a wave)
+  const int64_t groups = B * Hkv * p.tiles;
+  int64_t keys = (max_ctx * groups + 1023) / 1024;
+  keys = (keys + 127) / 128 * 128;
+  if (keys < 128) keys = 128;
+  p.split_keys = (int)(keys > 2048 ? 2048 : keys);
+  if (groups >= 1024) p.split_keys = (int)((max_ctx + 127) / 128 * 128);
+  p.splits = (int)((max_ctx + p.split_keys - 1) / p.split_keys);
+  return p;
 }
 
 inline bool odd16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
@@ -194,8 +463,10 @@ extern "C" int zk_kv_append_paged(const void* qkv, const float* cos_t, const flo
 extern "C" int zk_attn_paged_ws(int64_t B, int64_t T, int64_t max_q, int64_t max_ctx, int64_t Hq, int64_t Hkv,
                                 int64_t head_dim, int64_t* ws_floats) {
   if (!ws_floats || B <= 0 || T < 0 || max_q <= 0 || max_ctx <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv) return ZK_EINVAL;
-  if (head_dim != 64 && head_dim != 128) return ZK_EINVAL;
-  *ws_floats = 0;
+  if ((head_dim != 64 && head_dim != 128) || T > 0x7FFFFFFF || max_q > 0x7FFFFFFF || max_ctx > 0x7FFFFF00) return ZK_EINVAL;
+  if (max_q * (Hq / Hkv) > 0x7FFFFFFF || B > 0x7FFFFFFE || T * Hq > 0x7FFFFFFF) return ZK_EINVAL;
+  const Plan p = plan_of(B, max_q, max_ctx, Hq, Hkv);
+  *ws_floats = p.splits > 1 ? T * Hq * p.splits * (head_dim + 2) : 0;
   return ZK_OK;
 }
 
@@ -217,11 +488,22 @@ extern "C" int zk_attn_paged(const void* q, const void* k_cache, const void* v_c
   if (odd16(q) || odd16(k_cache) || odd16(v_cache) || odd16(out) || (need > 0 && (!ws || odd16(ws) || ws_floats < need)))
     return ZK_EINVAL;
   if (T == 0) return ZK_OK;
+  const Plan p = plan_of(B, max_q, max_ctx, Hq, Hkv);
+  const int64_t groups = B * Hkv * p.tiles * p.splits;
+  if (groups > 0x7FFFFFFF) return ZK_EINVAL;
+  float* part_o = p.splits > 1 ? ws : nullptr;
   PagedArgs a{(const bf16_t*)q, (const bf16_t*)k_cache, (const bf16_t*)v_cache, (bf16_t*)out, page_table, ctx_lens, cu_q,
-              (const unsigned long long*)tree_mask, (int)T, (int)B, (int)Hq, (int)Hkv, (int)page_size, (int)n_pages,
-              (int)table_cols, (int)ld_table, (int)mask_words, (long long)ldq, (long long)ldo, scale};
-  auto kern = head_dim == 128 ? attn_paged_rows_kernel<128> : attn_paged_rows_kernel<64>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)(T * Hq)), dim3(64), 0, stream, a);
+              (const unsigned long long*)tree_mask, part_o, part_o ? ws + T * Hq * p.splits * head_dim : nullptr, (int)T,
+              (int)B, (int)Hq, (int)Hkv, (int)page_size, (int)n_pages, (int)table_cols, (int)ld_table, (int)mask_words,
+              p.tiles, p.splits, p.split_keys, (long long)ldq, (long long)ldo, scale};
+  void (*kern)(PagedArgs) =
+      head_dim == 128 ? (p.mt == 1 ? attn_paged_stream_kernel<128, 1> : p.mt == 2 ? attn_paged_stream_kernel<128, 2> : attn_paged_stream_kernel<128, 4>)
+                      : (p.mt == 1 ? attn_paged_stream_kernel<64, 1> : p.mt == 2 ? attn_paged_stream_kernel<64, 2> : attn_paged_stream_kernel<64, 4>);
+  hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(256), 0, stream, a);
+  if (p.splits > 1) {
+    void (*merge)(PagedArgs) = head_dim == 128 ? attn_paged_merge_kernel<128> : attn_paged_merge_kernel<64>;
+    hipLaunchKernelGGL(merge, dim3((unsigned)(T * Hq)), dim3((unsigned)head_dim), 0, stream, a);
+  }
   ZK_CHECK_LAUNCH();
   return ZK_OK;
 }
