@@ -6,12 +6,14 @@
 // and a contiguous cache [B][rows][Hkv * hd] is the special case of one page per sequence.
 // Every index that comes from device memory (slots, positions, page numbers, lengths) is checked in the kernel against
 // the sizes the host passed: nothing is read or written outside the arrays whatever the tables hold.
-#include "common.h"
+#include "attn_common.h"
 #include "../../include/zero_hip.h"
+
+using namespace zkattn;
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = LOG2E;
 
 // =========================================================================================
 // append: one workgroup per token, a unit of work is 16 values of a head (two 16-byte chunks) that turn by 8 angles.
@@ -90,7 +92,8 @@ struct PagedArgs {
   const unsigned long long* mask;
   float *part_o, *part_ml;      // [T * Hq][splits][HD] un-normalised outputs, [..][2] maximum and sum; null: one split
   int T, B, Hq, Hkv, page_size, n_pages, table_cols, ld_table, mask_words;
-  int tiles, splits, split_keys;
+  int tiles, splits, split_keys, groups;
+  unsigned page_mul, page_shift;   // key / page_size = key * page_mul >> page_shift for every key < 2^31
   long long ldq, ldo;
   float scale;
 };
@@ -127,9 +130,25 @@ __device__ __forceinline__ unsigned seen_bits(const PagedArgs& a, const Seq& s, 
 // flat cache row of key `key` of sequence b, or -1: past `end`, or on a page that does not exist
 __device__ __forceinline__ int cache_row(const PagedArgs& a, int b, int key, int end) {
   if (key >= end) return -1;
-  const unsigned pg = (unsigned)a.table[(size_t)b * a.ld_table + (unsigned)key / (unsigned)a.page_size];
-  return pg < (unsigned)a.n_pages ? (int)(pg * (unsigned)a.page_size + (unsigned)key % (unsigned)a.page_size) : -1;
+  const unsigned at = (unsigned)(((unsigned long long)(unsigned)key * a.page_mul) >> a.page_shift);
+  const unsigned pg = (unsigned)a.table[(size_t)b * a.ld_table + at];
+  return pg < (unsigned)a.n_pages ? (int)(pg * (unsigned)a.page_size + ((unsigned)key - at * (unsigned)a.page_size)) : -1;
 }
+
+// workgroup -> (sequence, kv head, share, row tile), tiles fastest; an XCD (workgroups id % 8) takes consecutive work, so
+// that the tiles that read the same keys find them in its L2
+struct Work {
+  int tile, split, kvh, b;
+  bool any;
+  __device__ __forceinline__ Work(const PagedArgs& a) {
+    int w = (int)(blockIdx.x & 7) * ((a.groups + 7) >> 3) + (int)(blockIdx.x >> 3);
+    any = w < a.groups && (int)(blockIdx.x >> 3) < ((a.groups + 7) >> 3);
+    tile = w % a.tiles; w /= a.tiles;
+    split = w % a.splits; w /= a.splits;
+    kvh = w % a.Hkv;
+    b = w / a.Hkv;
+  }
+};
 
 __device__ __forceinline__ bool not_finite(unsigned w) {
   return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
@@ -151,7 +170,7 @@ struct Merge {
 };
 
 template <int HD, int MT>
-__global__ __launch_bounds__(256, MT == 1 ? (HD == 128 ? 3 : 4) : MT == 2 ? 2 : 1) void attn_paged_stream_kernel(PagedArgs a) {
+__global__ __launch_bounds__(256, MT == 1 ? (HD == 128 ? 3 : 4) : 2) void attn_paged_stream_kernel(PagedArgs a) {
   constexpr int CPR = HD / 8, KC = HD / 32, DB = HD / 16, NV = HD / 16, LDO = Merge<HD>::LDO;
   constexpr int VB = 32 * HD * 2;                   // one wave's V piece
   constexpr int XB = 4 * 16 * LDO * 4;
@@ -159,11 +178,9 @@ __global__ __launch_bounds__(256, MT == 1 ? (HD == 128 ? 3 : 4) : MT == 2 ? 2 : 
   __shared__ float sm[4][16 * MT], sl[4][16 * MT];
   const int tid = threadIdx.x, lane = tid & 63, g4 = lane >> 4, col = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int id = blockIdx.x;
-  const int kvh = id % a.Hkv; id /= a.Hkv;
-  const int tile = id % a.tiles; id /= a.tiles;
-  const int split = id % a.splits;
-  const int b = id / a.splits;
+  const Work w(a);
+  if (!w.any) return;
+  const int kvh = w.kvh, tile = w.tile, split = w.split, b = w.b;
   const Seq s(a, b);
   const int G = a.Hq / a.Hkv, rows = s.n * G, r0 = tile * 16 * MT, kvw = a.Hkv * HD;
   const int ks = split * a.split_keys;
@@ -389,10 +406,208 @@ __global__ __launch_bounds__(256, MT == 1 ? (HD == 128 ? 3 : 4) : MT == 2 ? 2 : 
   }
 }
 
-// out = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the shares of a row's sequence, in order: one workgroup of
-// HD threads per (token, head)
+// =========================================================================================
+// the same for many rows (prompt chunks, large trees): a workgroup is 128 rows of one kv head, four waves of 32 rows that
+// share every 64-key tile.  K and V tiles arrive by LDS-DMA (per-lane 64-bit source addresses: the rows of a paged cache),
+// chunk-swizzled, two stages, one barrier per tile; S^T = K Q^T and O^T += V^T P^T in 32x32x16 MFMAs with the row on
+// the lane, as in zk_attn_fwd.  Bound by the matrix and vector pipes in turn; see that kernel's header.
+// =========================================================================================
+template <int HD>
+__global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedArgs a) {
+  using C = Cfg<HD>;
+  constexpr int KV = 64, RB = HD * 2, TB = KV * RB, STAGE = 2 * TB, CPR = HD / 8, NQ = KV * CPR / 256;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Work w(a);
+  if (!w.any) return;
+  const int kvh = w.kvh, b = w.b, split = w.split;
+  const Seq s(a, b);
+  const int G = a.Hq / a.Hkv, rows = s.n * G, kvw = a.Hkv * HD, t0 = w.tile * 128;
+  const int ks = split * a.split_keys;
+  if (t0 >= rows || (split > 0 && ks >= s.len)) return;
+  const int ke = split == a.splits - 1 ? s.len : min(s.len, ks + a.split_keys);
+  const bool alone = ks == 0 && ke == s.len;
+  const float sc = a.scale * kLog2e;
+  const int r0 = t0 + wave * 32, r = r0 + (lane & 31), rc = min(r, rows - 1), tok = rc / G;
+  // keys that the workgroup / this wave needs at all, and those that all of the wave's rows see
+  const long long last_wg = a.mask ? s.len : s.first + min(t0 + 127, rows - 1) / G + 1;
+  const long long last_wave = r0 >= rows ? 0 : a.mask ? s.len : s.first + min(r0 + 31, rows - 1) / G + 1;
+  const long long clear = s.first + (a.mask ? 0 : min(r0, rows - 1) / G + 1);
+  const int end = (int)min((long long)ke, max(last_wg, (long long)ks));
+  const int nt = (end - ks + KV - 1) / KV;
+  const bf16_t* kb = a.k + kvh * HD;
+  const bf16_t* vb = a.v + kvh * HD;
+
+  auto issue = [&](int t, int rr) __attribute__((always_inline)) {         // rr: cache row of key `lane` of tile t
+    unsigned char* st = smem + (t & 1) * STAGE;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      const int sidx = tid + 256 * i, trow = sidx / CPR, ch = (sidx % CPR) ^ swz_key<HD>(trow);
+      const size_t off = (size_t)max(__shfl(rr, trow, 64), 0) * kvw + ch * 8;
+      unsigned char* dst = st + (wave * 64 + 256 * i) * 16;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kb + off),
+                                       (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vb + off),
+                                       (__attribute__((address_space(3))) void*)(dst + TB), 16, 0, 0);
+    }
+  };
+  int row = cache_row(a, b, ks + lane, ke), next = -1;
+  if (nt > 0) {
+    issue(0, row);
+    next = cache_row(a, b, ks + KV + lane, ke);
+  }
+  bf16x8 qf[C::DS];
+  {
+    const bf16_t* qp = a.q + (size_t)(s.q0 + tok) * a.ldq + (size_t)(kvh * G + rc % G) * HD + 8 * h;
+#pragma unroll
+    for (int ds = 0; ds < C::DS; ++ds) qf[ds] = *reinterpret_cast<const bf16x8*>(qp + ds * 16);
+  }
+  f32x16 o[C::DB];
+#pragma unroll
+  for (int d = 0; d < C::DB; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+  float m_run = -INFINITY, l_run = 0.f;
+#pragma unroll
+  for (int ds = 0; ds < C::DS; ++ds) asm volatile("" ::"v"(qf[ds]));
+
+  for (int t = 0; t < nt; ++t) {
+    const int k0 = ks + t * KV;
+    const unsigned long long ok = __ballot(row >= 0);           // the same in every wave
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();                                            // tile t is here, tile t - 1 is consumed
+    const unsigned char* kl = smem + (t & 1) * STAGE;
+    const unsigned char* vl = kl + TB;
+    if (t + 1 < nt) {
+      row = next;
+      issue(t + 1, row);
+      next = cache_row(a, b, k0 + 2 * KV + lane, ke);
+    }
+    bool odd = false;
+    const bool edge_wg = k0 + KV > s.first || ok != ~0ull;      // uniform over the workgroup
+    if (edge_wg) {
+      // rows that do not exist are zeros in V (their p is 0, and 0 x NaN is not); infinities and NaN are looked for
+      bool mine = false;
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        const int sidx = tid + 256 * i, trow = sidx / CPR;
+        u32x4* x = reinterpret_cast<u32x4*>(const_cast<unsigned char*>(vl) + sidx * 16);
+        if (!((ok >> trow) & 1)) *x = u32x4{0u, 0u, 0u, 0u};
+        else {
+          const u32x4 y = *x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mine |= not_finite(y[e]);
+        }
+      }
+      odd = __syncthreads_or((int)mine) != 0;
+    }
+    if (k0 >= last_wave) continue;
+    f32x16 st[2];
+#pragma unroll
+    for (int kb2 = 0; kb2 < 2; ++kb2) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) st[kb2][e] = 0.f;
+#pragma unroll
+      for (int ds = 0; ds < C::DS; ++ds)
+        st[kb2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag_sw<HD>(kl, kb2 * 32, ds, lane), qf[ds], st[kb2], 0, 0, 0);
+    }
+    if (k0 + KV > clear || ok != ~0ull) {
+#pragma unroll
+      for (int kb2 = 0; kb2 < 2; ++kb2) {
+        const unsigned vis = seen_bits(a, s, tok, k0 + 32 * kb2) & (unsigned)(ok >> (32 * kb2));
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (!((vis >> acc_row(e, h)) & 1)) st[kb2][e] = -INFINITY;
+      }
+    }
+    float mx = fmaxf(st[0][0], st[1][0]);
+#pragma unroll
+    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, fmaxf(st[0][e], st[1][e]));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float mn = fmaxf(m_run, mx * sc);
+    const float use = mn == -INFINITY ? 0.f : mn;
+    const float f = fast_exp2(m_run - use);
+    float rs = 0.f;
+#pragma unroll
+    for (int kb2 = 0; kb2 < 2; ++kb2)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float x = fast_exp2(__builtin_fmaf(st[kb2][e], sc, -use));
+        st[kb2][e] = x;
+        rs += x;
+      }
+    l_run = l_run * f + rs;
+    m_run = mn;
+#pragma unroll
+    for (int d = 0; d < C::DB; ++d) o[d] = o[d] * f;
+    if (__builtin_expect(!odd, 1)) {
+#pragma unroll
+      for (int kb2 = 0; kb2 < 2; ++kb2)
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const bf16x8 pf = pack_acc(st[kb2], z);
+#pragma unroll
+          for (int d = 0; d < C::DB; ++d)
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_frag_sw<HD>(vl, kb2 * 32, z, d, lane), pf, o[d], 0, 0, 0);
+        }
+    } else {
+      // key by key, keys with p = 0 passed over
+#pragma unroll 1
+      for (int kk = 0; kk < KV; ++kk) {
+        float x = 0.f;
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (e == (kk >> 5) * 16 + (kk & 3) + 4 * ((kk & 31) >> 3)) x = st[e >> 4][e & 15];
+        x = (float)(__bf16)__shfl(x, ((kk >> 2) & 1) * 32 + (lane & 31), 64);
+        if (x == 0.f) continue;
+#pragma unroll
+        for (int d = 0; d < C::DB; ++d)
+#pragma unroll
+          for (int r4 = 0; r4 < 4; ++r4) {
+            const int ch = d * 4 + r4;
+            const u32x2 y = *reinterpret_cast<const u32x2*>(vl + kk * RB + ((ch ^ swz_key<HD>(kk)) << 4) + 8 * h);
+            o[d][4 * r4] += x * lo_bf(y[0]); o[d][4 * r4 + 1] += x * hi_bf(y[0]);
+            o[d][4 * r4 + 2] += x * lo_bf(y[1]); o[d][4 * r4 + 3] += x * hi_bf(y[1]);
+          }
+      }
+    }
+  }
+  const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
+  if (r >= rows) return;
+  const int tq = s.q0 + tok, head = kvh * G + rc % G;
+  if (alone) {
+    const float inv = l_tot > 0.f ? 1.0f / l_tot : (l_tot == 0.f ? 0.f : l_tot);
+    bf16_t* op = a.out + (size_t)tq * a.ldo + (size_t)head * HD;
+#pragma unroll
+    for (int d = 0; d < C::DB; ++d)
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        u32x2 y;
+        y[0] = pack2bf(o[d][4 * r4] * inv, o[d][4 * r4 + 1] * inv);
+        y[1] = pack2bf(o[d][4 * r4 + 2] * inv, o[d][4 * r4 + 3] * inv);
+        *reinterpret_cast<u32x2*>(op + d * 32 + 8 * r4 + 4 * h) = y;
+      }
+  } else {
+    const size_t part = ((size_t)tq * a.Hq + head) * a.splits + split;
+#pragma unroll
+    for (int d = 0; d < C::DB; ++d)
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4)
+        *reinterpret_cast<f32x4*>(a.part_o + part * HD + d * 32 + 8 * r4 + 4 * h) =
+            f32x4{o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]};
+    if (h == 0) { a.part_ml[part * 2] = m_run; a.part_ml[part * 2 + 1] = l_tot; }
+  }
+}
+
+// out = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the shares of a row's sequence, in a fixed order: one workgroup
+// per (token, head), four groups of HD / 4 threads take every fourth share and are added in order
 template <int HD>
 __global__ __launch_bounds__(HD) void attn_paged_merge_kernel(PagedArgs a) {
+  constexpr int TPG = HD / 4, NG = 4;
+  __shared__ float wgt[1024];
+  __shared__ __attribute__((aligned(16))) float acc[NG][HD];
+  __shared__ float red[4];
   const int t = blockIdx.x / a.Hq, h = blockIdx.x % a.Hq, d = threadIdx.x;
   int lo = 0, hi = a.B;                             // last sequence that starts at or before row t
   while (hi - lo > 1) {
@@ -403,36 +618,63 @@ __global__ __launch_bounds__(HD) void attn_paged_merge_kernel(PagedArgs a) {
   if (t < s.q0 || t >= s.q0 + s.n) return;
   const int parts = min(a.splits, (s.len + a.split_keys - 1) / a.split_keys);
   if (parts <= 1) return;                           // written by its only share
-  const size_t p0 = (size_t)blockIdx.x * a.splits;
+  const float* ml = a.part_ml + (size_t)blockIdx.x * a.splits * 2;
+  const float* po = a.part_o + (size_t)blockIdx.x * a.splits * HD;
   float M = -INFINITY;
-  for (int i = 0; i < parts; ++i) M = fmaxf(M, a.part_ml[(p0 + i) * 2]);
-  float L = 0.f, y = 0.f;
-  for (int i = 0; i < parts; ++i) {
-    const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(a.part_ml[(p0 + i) * 2] - M);
-    L += a.part_ml[(p0 + i) * 2 + 1] * f;
-    y += a.part_o[(p0 + i) * HD + d] * f;
+  for (int i = d; i < parts; i += HD) M = fmaxf(M, ml[2 * i]);
+  M = wave_max(M);
+  if ((d & 63) == 0) red[d >> 6] = M;
+  __syncthreads();
+  for (int i = 0; i < HD / 64; ++i) M = fmaxf(M, red[i]);
+  const int g = d / TPG, c = (d % TPG) * 4;
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+  float L = 0.f;
+  for (int i0 = 0; i0 < parts; i0 += 1024) {
+    const int np = min(1024, parts - i0);
+    __syncthreads();
+    for (int i = d; i < np; i += HD) {
+      const float f = M == -INFINITY ? 0.f : fast_exp2(ml[2 * (i0 + i)] - M);
+      wgt[i] = f;
+      L += ml[2 * (i0 + i) + 1] * f;
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int i = g; i < np; i += NG) {
+      // a share that saw nothing of this row has weight 0 and an output of zeros
+      const f32x4 x = *reinterpret_cast<const f32x4*>(po + (size_t)(i0 + i) * HD + c);
+      y += x * wgt[i];
+    }
   }
+  *reinterpret_cast<f32x4*>(&acc[g][c]) = y;
+  L = wave_sum(L);
+  __syncthreads();
+  if ((d & 63) == 0) red[d >> 6] = L;
+  __syncthreads();
+  L = 0.f;
+  for (int i = 0; i < HD / 64; ++i) L += red[i];
   const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
-  a.out[(size_t)t * a.ldo + (size_t)h * HD + d] = f2bf(y * inv);
+  a.out[(size_t)t * a.ldo + (size_t)h * HD + d] = f2bf(((acc[0][d] + acc[1][d]) + (acc[2][d] + acc[3][d])) * inv);
 }
 
 // shape of a launch: host arithmetic on the sizes alone
 struct Plan {
-  int mt, tiles, splits, split_keys;
+  int mt, tiles, splits, split_keys;                // mt: 16-row groups of the stream kernel's tile, 8 = the tile kernel
 };
 inline Plan plan_of(int64_t B, int64_t max_q, int64_t max_ctx, int64_t Hq, int64_t Hkv) {
   Plan p;
   const int64_t rows = max_q * (Hq / Hkv);
-  p.mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  p.mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 8;
   p.tiles = (int)((rows + 16 * p.mt - 1) / (16 * p.mt));
-  // shares of the keys: enough workgroups for four rounds of the 256 CUs, none under 128 keys (one piece a wave)
+  // shares of the keys: enough workgroups for two rounds of what the 256 CUs hold at two a CU, none under 128 keys (one
+  // piece a wave), and none over 2048 while there are fewer groups than that
   const int64_t groups = B * Hkv * p.tiles;
   int64_t keys = (max_ctx * groups + 1023) / 1024;
   keys = (keys + 127) / 128 * 128;
   if (keys < 128) keys = 128;
-  p.split_keys = (int)(keys > 2048 ? 2048 : keys);
-  if (groups >= 1024) p.split_keys = (int)((max_ctx + 127) / 128 * 128);
-  p.splits = (int)((max_ctx + p.split_keys - 1) / p.split_keys);
+  if (keys > 2048 && groups < 512) keys = 2048;
+  if (groups >= 512) keys = (max_ctx + 127) / 128 * 128;
+  p.split_keys = (int)keys;
+  p.splits = (int)((max_ctx + keys - 1) / keys);
   return p;
 }
 
@@ -490,16 +732,19 @@ extern "C" int zk_attn_paged(const void* q, const void* k_cache, const void* v_c
   if (T == 0) return ZK_OK;
   const Plan p = plan_of(B, max_q, max_ctx, Hq, Hkv);
   const int64_t groups = B * Hkv * p.tiles * p.splits;
-  if (groups > 0x7FFFFFFF) return ZK_EINVAL;
+  if (groups > 0x7FFFFFF0) return ZK_EINVAL;
+  int lg = 0;                                       // page_mul: the 31-bit reciprocal, rounded up (exact below 2^31)
+  while ((int64_t)1 << lg < page_size) ++lg;
+  const unsigned mul = (unsigned)((((unsigned long long)1 << (31 + lg)) / (unsigned long long)page_size) + 1);
   float* part_o = p.splits > 1 ? ws : nullptr;
   PagedArgs a{(const bf16_t*)q, (const bf16_t*)k_cache, (const bf16_t*)v_cache, (bf16_t*)out, page_table, ctx_lens, cu_q,
               (const unsigned long long*)tree_mask, part_o, part_o ? ws + T * Hq * p.splits * head_dim : nullptr, (int)T,
               (int)B, (int)Hq, (int)Hkv, (int)page_size, (int)n_pages, (int)table_cols, (int)ld_table, (int)mask_words,
-              p.tiles, p.splits, p.split_keys, (long long)ldq, (long long)ldo, scale};
+              p.tiles, p.splits, p.split_keys, (int)groups, mul, (unsigned)(31 + lg), (long long)ldq, (long long)ldo, scale};
   void (*kern)(PagedArgs) =
-      head_dim == 128 ? (p.mt == 1 ? attn_paged_stream_kernel<128, 1> : p.mt == 2 ? attn_paged_stream_kernel<128, 2> : attn_paged_stream_kernel<128, 4>)
-                      : (p.mt == 1 ? attn_paged_stream_kernel<64, 1> : p.mt == 2 ? attn_paged_stream_kernel<64, 2> : attn_paged_stream_kernel<64, 4>);
-  hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(256), 0, stream, a);
+      head_dim == 128 ? (p.mt == 1 ? attn_paged_stream_kernel<128, 1> : p.mt == 2 ? attn_paged_stream_kernel<128, 2> : attn_paged_tile_kernel<128>)
+                      : (p.mt == 1 ? attn_paged_stream_kernel<64, 1> : p.mt == 2 ? attn_paged_stream_kernel<64, 2> : attn_paged_tile_kernel<64>);
+  hipLaunchKernelGGL(kern, dim3((unsigned)((groups + 7) / 8 * 8)), dim3(256), 0, stream, a);
   if (p.splits > 1) {
     void (*merge)(PagedArgs) = head_dim == 128 ? attn_paged_merge_kernel<128> : attn_paged_merge_kernel<64>;
     hipLaunchKernelGGL(merge, dim3((unsigned)(T * Hq)), dim3((unsigned)head_dim), 0, stream, a);
