@@ -430,10 +430,9 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedArgs a) {
   const bool alone = ks == 0 && ke == s.len;
   const float sc = a.scale * kLog2e;
   const int r0 = t0 + wave * 32, r = r0 + (lane & 31), rc = min(r, rows - 1), tok = rc / G;
-  // keys that the workgroup / this wave needs at all, and those that all of the wave's rows see
+  // keys that the workgroup / this wave needs at all
   const long long last_wg = a.mask ? s.len : s.first + min(t0 + 127, rows - 1) / G + 1;
   const long long last_wave = r0 >= rows ? 0 : a.mask ? s.len : s.first + min(r0 + 31, rows - 1) / G + 1;
-  const long long clear = s.first + (a.mask ? 0 : min(r0, rows - 1) / G + 1);
   const int end = (int)min((long long)ke, max(last_wg, (long long)ks));
   const int nt = (end - ks + KV - 1) / KV;
   const bf16_t* kb = a.k + kvh * HD;
@@ -472,55 +471,31 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedArgs a) {
 #pragma unroll
   for (int ds = 0; ds < C::DS; ++ds) asm volatile("" ::"v"(qf[ds]));
 
-  for (int t = 0; t < nt; ++t) {
-    const int k0 = ks + t * KV;
-    const unsigned long long ok = __ballot(row >= 0);           // the same in every wave
+  f32x16 st[2];
+  int t = 0;
+  const unsigned char *kl, *vl;
+  auto landed = [&]() __attribute__((always_inline)) {           // tile t is here, tile t - 1 is consumed: its stage takes t + 1
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();                                            // tile t is here, tile t - 1 is consumed
-    const unsigned char* kl = smem + (t & 1) * STAGE;
-    const unsigned char* vl = kl + TB;
+    __syncthreads();
+    kl = smem + (t & 1) * STAGE;
+    vl = kl + TB;
+    row = next;
     if (t + 1 < nt) {
-      row = next;
       issue(t + 1, row);
-      next = cache_row(a, b, k0 + 2 * KV + lane, ke);
+      next = cache_row(a, b, ks + (t + 2) * KV + lane, ke);
     }
-    bool odd = false;
-    const bool edge_wg = k0 + KV > s.first || ok != ~0ull;      // uniform over the workgroup
-    if (edge_wg) {
-      // rows that do not exist are zeros in V (their p is 0, and 0 x NaN is not); infinities and NaN are looked for
-      bool mine = false;
+  };
+  auto scores = [&]() __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) {
-        const int sidx = tid + 256 * i, trow = sidx / CPR;
-        u32x4* x = reinterpret_cast<u32x4*>(const_cast<unsigned char*>(vl) + sidx * 16);
-        if (!((ok >> trow) & 1)) *x = u32x4{0u, 0u, 0u, 0u};
-        else {
-          const u32x4 y = *x;
+    for (int x = 0; x < 2; ++x) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mine |= not_finite(y[e]);
-        }
-      }
-      odd = __syncthreads_or((int)mine) != 0;
-    }
-    if (k0 >= last_wave) continue;
-    f32x16 st[2];
-#pragma unroll
-    for (int kb2 = 0; kb2 < 2; ++kb2) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) st[kb2][e] = 0.f;
+      for (int e = 0; e < 16; ++e) st[x][e] = 0.f;
 #pragma unroll
       for (int ds = 0; ds < C::DS; ++ds)
-        st[kb2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag_sw<HD>(kl, kb2 * 32, ds, lane), qf[ds], st[kb2], 0, 0, 0);
+        st[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag_sw<HD>(kl, x * 32, ds, lane), qf[ds], st[x], 0, 0, 0);
     }
-    if (k0 + KV > clear || ok != ~0ull) {
-#pragma unroll
-      for (int kb2 = 0; kb2 < 2; ++kb2) {
-        const unsigned vis = seen_bits(a, s, tok, k0 + 32 * kb2) & (unsigned)(ok >> (32 * kb2));
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (!((vis >> acc_row(e, h)) & 1)) st[kb2][e] = -INFINITY;
-      }
-    }
+  };
+  auto softmax = [&]() __attribute__((always_inline)) {
     float mx = fmaxf(st[0][0], st[1][0]);
 #pragma unroll
     for (int e = 1; e < 16; ++e) mx = fmaxf(mx, fmaxf(st[0][e], st[1][e]));
@@ -530,27 +505,70 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedArgs a) {
     const float f = fast_exp2(m_run - use);
     float rs = 0.f;
 #pragma unroll
-    for (int kb2 = 0; kb2 < 2; ++kb2)
+    for (int x = 0; x < 2; ++x)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const float x = fast_exp2(__builtin_fmaf(st[kb2][e], sc, -use));
-        st[kb2][e] = x;
-        rs += x;
+        const float p = fast_exp2(__builtin_fmaf(st[x][e], sc, -use));
+        st[x][e] = p;
+        rs += p;
       }
     l_run = l_run * f + rs;
     m_run = mn;
 #pragma unroll
     for (int d = 0; d < C::DB; ++d) o[d] = o[d] * f;
-    if (__builtin_expect(!odd, 1)) {
+  };
+  auto product = [&]() __attribute__((always_inline)) {
 #pragma unroll
-      for (int kb2 = 0; kb2 < 2; ++kb2)
+    for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const bf16x8 pf = pack_acc(st[kb2], z);
+      for (int z = 0; z < 2; ++z) {
+        const bf16x8 pf = pack_acc(st[x], z);
 #pragma unroll
-          for (int d = 0; d < C::DB; ++d)
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_frag_sw<HD>(vl, kb2 * 32, z, d, lane), pf, o[d], 0, 0, 0);
-        }
+        for (int d = 0; d < C::DB; ++d)
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_frag_sw<HD>(vl, x * 32, z, d, lane), pf, o[d], 0, 0, 0);
+      }
+  };
+  // tiles that every row of the workgroup sees whole
+  const long long clear_wg = min((long long)ke, s.first + (a.mask ? 0 : t0 / G + 1)) - ks;
+  const int bulk = clear_wg < KV ? 0 : (int)(clear_wg / KV);
+  while (t < bulk && __all(row >= 0)) {
+    landed();
+    scores();
+    softmax();
+    product();
+    ++t;
+  }
+  // the others: the cache's end, new tokens, pages that do not exist (and what stands behind one)
+  for (; t < nt; ++t) {
+    const int k0 = ks + t * KV;
+    const unsigned long long ok = __ballot(row >= 0);           // the same in every wave
+    landed();
+    // rows that do not exist are zeros in V (their p is 0, and 0 x NaN is not); infinities and NaN are looked for
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      const int sidx = tid + 256 * i;
+      u32x4* x = reinterpret_cast<u32x4*>(const_cast<unsigned char*>(vl) + sidx * 16);
+      if (!((ok >> (sidx / CPR)) & 1)) *x = u32x4{0u, 0u, 0u, 0u};
+      else {
+        const u32x4 y = *x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) odd |= not_finite(y[e]);
+      }
+    }
+    const bool any_odd = __syncthreads_or((int)odd) != 0;
+    if (k0 >= last_wave) continue;
+    scores();
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const unsigned vis = seen_bits(a, s, tok, k0 + 32 * x) & (unsigned)(ok >> (32 * x));
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (!((vis >> acc_row(e, h)) & 1)) st[x][e] = -INFINITY;
+    }
+    softmax();
+    if (!any_odd) {
+      product();
     } else {
       // key by key, keys with p = 0 passed over
 #pragma unroll 1
