@@ -40,40 +40,53 @@ struct SampleArgs {
   long long V, ld;
 };
 
-// place of a logit in falling order (0 = largest): -0 is +0.  0x7F = +inf, 0xFF80 = -inf; beyond these: NaN
-__device__ __forceinline__ int falling(unsigned b) {
-  const unsigned m = b & 0x7FFFu;
-  return (b & 0x8000u) && m ? (int)(0x7FFFu + m) : (int)(0x7FFFu - m);
+// A logit's key: its sign-magnitude bits as a two's complement number, so that keys are in the logits' order and -0 is +0.
+// +inf 0x7F80, -inf -0x7F80, beyond these: NaN.  Two keys to a register, as the logits come: packed 16-bit instructions
+// make them, find the largest and count matches, at one to two instructions a token (a single workgroup has 16 waves for
+// 10^5 tokens: every instruction per token is 2 us of the 20).
+typedef __attribute__((ext_vector_type(2))) short s16x2;
+constexpr int kInf = 0x7F80;
+__device__ __forceinline__ unsigned keys_of(unsigned w) {
+  const s16x2 m = __builtin_bit_cast(s16x2, w) >> (s16x2)15;
+  return __builtin_bit_cast(unsigned, (s16x2)((__builtin_bit_cast(s16x2, w & 0x7FFF7FFFu) ^ m) - m));
 }
-constexpr int kTop = 0x7F, kBottom = 0x7FFF + 0x7F80;   // +inf, -inf
-__device__ __forceinline__ double value_of(int d) {
-  const unsigned b = d <= 0x7FFF ? (unsigned)(0x7FFF - d) : (0x8000u | (unsigned)(d - 0x7FFF));
-  return (double)bf2f((bf16_t)b);
+__device__ __forceinline__ double value_of(int key) {
+  return (double)bf2f((bf16_t)(key < 0 ? 0x8000u | (unsigned)-key : (unsigned)key));
 }
 
 struct Row {
-  u32x4 r[kChunks];
-  // chunk c of the part: tokens part + (c * kThreads + tid) * 8 - skew .., where skew makes the address 16-byte aligned
-  __device__ __forceinline__ void load(const bf16_t* row, long long V, long long part, int skew, int tid) {
+  u32x4 r[kChunks];                                 // keys
+  // chunk c of the part: tokens part + (c * kThreads + tid) * 8 - skew .., where skew makes the address 16-byte aligned;
+  // `n` tokens (and skew) are left from `part` on
+  __device__ __forceinline__ void load(const bf16_t* row, long long part, int n, int skew, int tid) {
+    const bf16_t* p = row + part - skew;
+    const int lo = part ? 0 : skew;                 // valid places of the part: [lo, n)
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
-      const long long i = part + (long long)(c * kThreads + tid) * 8 - skew;
       u32x4 x = {0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u};     // -inf outside the row
-      if (i >= 0 && i + 8 <= V) {
-        x = *reinterpret_cast<const u32x4*>(row + i);
-      } else if (i + 8 > 0 && i < V) {
+      if (c * kThreads * 8 < n) {
+        const int i = (c * kThreads + tid) * 8;
+        if (i >= lo && i + 8 <= n) {
+          x = *reinterpret_cast<const u32x4*>(p + i);
+        } else if (i + 8 > lo && i < n) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (i + e >= 0 && i + e < V) {
-            const unsigned v = row[i + e];
-            x[e >> 1] = e & 1 ? (x[e >> 1] & 0xFFFFu) | (v << 16) : (x[e >> 1] & 0xFFFF0000u) | v;
-          }
+          for (int e = 0; e < 8; ++e)
+            if (i + e >= lo && i + e < n) {
+              const unsigned v = p[i + e];
+              x[e >> 1] = e & 1 ? (x[e >> 1] & 0xFFFFu) | (v << 16) : (x[e >> 1] & 0xFFFF0000u) | v;
+            }
+        }
       }
       r[c] = x;
     }
   }
-  __device__ __forceinline__ int place(int c, int e) const {
-    return falling((r[c][e >> 1] >> ((e & 1) * 16)) & 0xFFFFu);
+  __device__ __forceinline__ void to_keys(int n) {
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c)
+      if (c * kThreads * 8 < n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[c][e] = keys_of(r[c][e]);
+      }
   }
 };
 
@@ -94,17 +107,16 @@ __device__ __forceinline__ T wave_upto(T v) {
   v += dpp0<0x143, 0xC>(v);
   return v;
 }
-__device__ __forceinline__ double from_lane(double v, int lane) {
-  return __hiloint2double(__shfl(__double2hiint(v), lane, 64), __shfl(__double2loint(v), lane, 64));
+__device__ __forceinline__ double lane_of(double v, int lane) {     // lane: the same in the whole wave
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane), __builtin_amdgcn_readlane(__double2loint(v), lane));
 }
-__device__ __forceinline__ int from_lane(int v, int lane) { return __shfl(v, lane, 64); }
+__device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
-// Sums over the bins in order (block, thread) of each thread's five: before[j] = all earlier ones, upto[j] = with this one
-// (the same bits as the next one's `before`, so exactly one holds a border); returns the total.  Fixed order.
+// Sums over the bins in order (block, thread) of each thread's five: before[j] = all earlier ones, upto[j] = with this one;
+// returns the total.  Fixed order.
 template <class T>
 __device__ __forceinline__ T running(const T (&v)[kBlocks], T (&before)[kBlocks], T (&upto)[kBlocks], T* ends) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  __syncthreads();
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
   for (int j = 0; j < kBlocks; ++j) {
     upto[j] = wave_upto(v[j]);
@@ -113,85 +125,98 @@ __device__ __forceinline__ T running(const T (&v)[kBlocks], T (&before)[kBlocks]
   __syncthreads();
   // ends[0 .. 79] -> their own running sums, in every wave by itself
   const T e0 = wave_upto(ends[lane]);
-  const T t0 = from_lane(e0, 63);
-  const T e1 = wave_upto(lane < kBlocks * kWaves - 64 ? ends[64 + lane] : T(0)) + t0;
+  const T e1 = wave_upto(lane < kBlocks * kWaves - 64 ? ends[64 + lane] : T(0)) + lane_of(e0, 63);
 #pragma unroll
   for (int j = 0; j < kBlocks; ++j) {
     const int at = j * kWaves + wave - 1;           // the wave before, in order
-    const T base = at < 0 ? T(0) : at < 64 ? from_lane(e0, at) : from_lane(e1, at - 64);
-    const T prev = from_lane(upto[j], lane ? lane - 1 : 0);
-    before[j] = base + (lane ? prev : T(0));
-    upto[j] = lane == 63 ? (at + 1 < 64 ? from_lane(e0, at + 1) : from_lane(e1, at + 1 - 64)) : base + upto[j];
+    const T base = at < 0 ? T(0) : at < 64 ? lane_of(e0, at & 63) : lane_of(e1, at & 63);
+    before[j] = base + dpp0<0x138, 0xF>(upto[j]);   // the lane before; lane 0: nothing
+    upto[j] = base + upto[j];
   }
-  return from_lane(e1, kBlocks * kWaves - 64 - 1);
+  return lane_of(e1, kBlocks * kWaves - 64 - 1);
 }
 
+// RESIDENT: the row fits a workgroup's registers (131 072 tokens, less what its address is past 16 bytes) and is read once;
+// otherwise each pass over the row reads it again, part by part.
+template <bool RESIDENT>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   __shared__ __attribute__((aligned(16))) unsigned hist[kBins];
-  __shared__ double ends_d[kBlocks * kWaves], hit_mass;
-  __shared__ int ends_i[kBlocks * kWaves], wtop[kWaves], wnan[kWaves], hit, hit_count;
+  __shared__ double ends_d[kBlocks * kWaves], mp_d[kWaves], cand_mass[3][kWaves], kept[3];
+  __shared__ int ends_i[kBlocks * kWaves], cand[3][kWaves], cand_count[kWaves], wtop[kWaves], wlow[kWaves], picked[2];
   __shared__ __attribute__((aligned(16))) unsigned matches[kChunks * kWaves];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const long long b = blockIdx.x;
   const bf16_t* row = a.logits + b * a.ld;
   const int skew = (int)((reinterpret_cast<uintptr_t>(row) & 15) >> 1);
   const long long span = a.V + skew;
+  auto left = [&](long long part) { return RESIDENT ? (int)span : (int)min(span - part, (long long)kRound); };
   Row x;
-  const bool resident = span <= kRound;
-  if (resident) x.load(row, a.V, 0, skew, tid);
+  if (RESIDENT) x.load(row, 0, left(0), skew, tid);
   float Tf = a.temperature_rows ? a.temperature_rows[b] : a.temperature;
   const int top_k = a.top_k_rows ? a.top_k_rows[b] : a.top_k;
   const double top_p = a.top_p_rows ? a.top_p_rows[b] : a.top_p;
   const double min_p = a.min_p_rows ? a.min_p_rows[b] : a.min_p;
+  const float u = a.u[b];
   const bool first_only = !(Tf > 0.f) || top_k == 1;      // the largest logit: nothing to count
   Tf = fminf(Tf, kMaxTemperature);
   if (!first_only)
     for (int i = tid; i < kBins / 4; i += kThreads) reinterpret_cast<u32x4*>(hist)[i] = u32x4{0u, 0u, 0u, 0u};
   // the largest logit, and whether any is NaN
-  int top = kBottom, low = kTop;
-  for (long long part = 0; part < span; part += kRound) {
-    if (!resident) x.load(row, a.V, part, skew, tid);
+  s16x2 hi2 = {-32768, -32768}, lo2 = {32767, 32767};
+  for (long long part = 0; part < (RESIDENT ? 1 : span); part += kRound) {
+    if (!RESIDENT) x.load(row, part, left(part), skew, tid);
+    x.to_keys(left(part));
 #pragma unroll
     for (int c = 0; c < kChunks; ++c)
+      if (c * kThreads * 8 < left(part)) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int d = x.place(c, e);
-        top = min(top, d);
-        low = max(low, d);
+        for (int e = 0; e < 4; ++e) {
+          const unsigned w = x.r[c][e];             // (a bit cast of a vector's element takes the vector's first one)
+          hi2 = __builtin_elementwise_max(hi2, __builtin_bit_cast(s16x2, w));
+          lo2 = __builtin_elementwise_min(lo2, __builtin_bit_cast(s16x2, w));
+        }
       }
   }
+  int top = max((int)hi2[0], (int)hi2[1]), low = min((int)lo2[0], (int)lo2[1]);
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) { top = min(top, __shfl_xor(top, o, 64)); low = max(low, __shfl_xor(low, o, 64)); }
-  if (lane == 0) { wtop[wave] = top; wnan[wave] = low; }
+  for (int o = 32; o > 0; o >>= 1) { top = max(top, __shfl_xor(top, o, 64)); low = min(low, __shfl_xor(low, o, 64)); }
+  if (lane == 0) { wtop[wave] = top; wlow[wave] = low; }
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) { top = min(top, wtop[w]); low = max(low, wnan[w]); }
-  const bool nan = top < kTop || low > kBottom;
-  if (nan || top >= kBottom) {                      // a NaN, or no token that can be drawn
+  for (int w = 0; w < kWaves; ++w) { top = max(top, wtop[w]); low = min(low, wlow[w]); }
+  const bool nan = top > kInf || low < -kInf;
+  if (nan || top == -kInf) {                        // a NaN, or no token that can be drawn
     if (tid == 0) {
       a.tokens[b] = -1;
       a.logprobs[b] = nan ? __builtin_nanf("") : -INFINITY;
     }
     return;
   }
+  top = __builtin_amdgcn_readfirstlane(top);
   int bin = 0, rank = 0;
-  double logp = 0.0;
   if (!first_only) {
-    for (long long part = 0; part < span; part += kRound) {
-      if (!resident) x.load(row, a.V, part, skew, tid);
+    // bin d counts the tokens of key top - d (a byte offset is 4 (top - key): one multiply-add; -inf has no weight)
+    const int top4 = top * 4;
+    for (long long part = 0; part < (RESIDENT ? 1 : span); part += kRound) {
+      if (!RESIDENT) { x.load(row, part, left(part), skew, tid); x.to_keys(left(part)); }
 #pragma unroll
       for (int c = 0; c < kChunks; ++c)
+        if (c * kThreads * 8 < left(part)) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int d = x.place(c, e) - top;
-          if (d < kBins && d < kBottom - top) atomicAdd(&hist[d], 1u);
+          for (int e = 0; e < 4; ++e) {
+            unsigned d0, d1;
+            asm("v_mad_i32_i16 %0, %1, %2, %3" : "=v"(d0) : "v"(x.r[c][e]), "v"(-4), "v"(top4));
+            asm("v_mad_i32_i16 %0, %1, %2, %3 op_sel:[1,0,0,0]" : "=v"(d1) : "v"(x.r[c][e]), "v"(-4), "v"(top4));
+            if (d0 < kBins * 4u) atomicAdd(reinterpret_cast<unsigned*>(reinterpret_cast<unsigned char*>(hist) + d0), 1u);
+            if (d1 < kBins * 4u) atomicAdd(reinterpret_cast<unsigned*>(reinterpret_cast<unsigned char*>(hist) + d1), 1u);
+          }
         }
     }
     __syncthreads();
     // weight of bin i (a maximum of +inf has the only weight)
     const double vtop = value_of(top), inv_t = 1.0 / (double)Tf;
     auto weight = [&](int i) {
-      const double z = (value_of(top + i) - vtop) * inv_t;
+      const double z = (value_of(top - i) - vtop) * inv_t;
       return i == 0 ? 1.0 : z > kNothing ? exp(z) : 0.0;
     };
     int cnt[kBlocks];
@@ -214,39 +239,43 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
         if (!(w < min_p)) mass_mp += cw;
       }
     }
+    mass_mp = wave_upto(mass_mp);
+    if (lane == 63) mp_d[wave] = mass_mp;
     double before[kBlocks], upto[kBlocks];
     const double total = running(mass, before, upto, ends_d);
     double Z = total;
-    // one thread's eight bins, on lanes 0 .. 7 of every wave: count, weight, and the sum before each from `from` on
-    int c8;
-    double w8, run8;
+    // Borders.  Each wave names its first eight bins, in order, that hold weight and whose running sum passes the border;
+    // the first of these resolves it: its bins on lanes 0 .. 7 of wave 0, count, weight and running sum each.
+    int c8 = 0;
+    double w8 = 0.0, run8 = 0.0;
     auto spread = [&](int at, double from) {
-      const int i = at * kRun + (lane & 7);       // thread t of block j: at = j * kThreads + t
+      const int i = at * kRun + (lane & 7);         // thread t of block j: at = j * kThreads + t
       c8 = (int)hist[i];
       w8 = c8 ? weight(i) : 0.0;
       double v = (double)c8 * w8;
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) {
-        const double y = from_lane(v, lane >= o ? lane - o : 0);
-        if ((lane & 7) >= o) v += y;
-      }
+      v += dpp0<0x111, 0xF>(v) * (double)((lane & 7) >= 1);
+      v += dpp0<0x112, 0xF>(v) * (double)((lane & 7) >= 2);
+      v += dpp0<0x114, 0xF>(v) * (double)((lane & 7) >= 4);
       run8 = from + v - (double)c8 * w8;
     };
-    // the first eight bins, in order, that hold weight and whose running sum passes a border
-    auto find = [&](auto passes) {
-      if (tid == 0) hit = 0x7FFFFFFF;
-      __syncthreads();
+    auto find = [&](int k, auto passes) {           // -> which eight bins, in wave 0
 #pragma unroll
-      for (int j = 0; j < kBlocks; ++j) {
+      for (int j = kBlocks - 1; j >= 0; --j) {
         const unsigned long long any = __ballot(mass[j] > 0.0 && passes(upto[j]));
-        if (any && lane == __ffsll(any) - 1) atomicMin(&hit, j * kThreads + tid);
+        if (j == kBlocks - 1 && lane == 0) cand[k][wave] = 0x7FFFFFFF;
+        if (any && lane == __ffsll(any) - 1) { cand[k][wave] = j * kThreads + tid; cand_mass[k][wave] = before[j]; }
       }
       __syncthreads();
+      int at = 0;
+      if (wave == 0) {
+        const int mine = lane < kWaves ? cand[k][lane] : 0x7FFFFFFF;
+        int best = mine;
 #pragma unroll
-      for (int j = 0; j < kBlocks; ++j)
-        if (hit == j * kThreads + tid) hit_mass = before[j];
-      __syncthreads();
-      spread(hit, hit_mass);
+        for (int o = 8; o > 0; o >>= 1) best = min(best, __shfl_xor(best, o, 64));
+        at = __builtin_amdgcn_readfirstlane(best);
+        spread(at, cand_mass[k][__ffsll(__ballot(mine == at)) - 1]);
+      }
+      return at;
     };
     // top-k: the sum of the first top_k
     if (top_k > 0) {
@@ -254,64 +283,78 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
       if (running(cnt, cnt_before, cnt_upto, ends_i) > top_k) {
 #pragma unroll
         for (int j = 0; j < kBlocks; ++j)
-          if (cnt_before[j] < top_k && top_k <= cnt_upto[j]) { hit = j * kThreads + tid; hit_count = cnt_before[j]; hit_mass = before[j]; }
+          if (cnt_before[j] < top_k && top_k <= cnt_upto[j]) { cand[0][0] = j * kThreads + tid; cand_count[0] = cnt_before[j]; cand_mass[0][0] = before[j]; }
         __syncthreads();
-        spread(hit, hit_mass);
-        int n = c8;
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) {
-          const int y = from_lane(n, lane >= o ? lane - o : 0);
-          if ((lane & 7) >= o) n += y;
+        if (wave == 0) {
+          spread(cand[0][0], cand_mass[0][0]);
+          int n = c8;
+          n += dpp0<0x111, 0xF>(n) * (int)((lane & 7) >= 1);
+          n += dpp0<0x112, 0xF>(n) * (int)((lane & 7) >= 2);
+          n += dpp0<0x114, 0xF>(n) * (int)((lane & 7) >= 4);
+          const int k = top_k - (cand_count[0] + n - c8);     // of this bin and later ones
+          if (lane == __ffsll(__ballot(lane < 8 && c8 > 0 && k <= c8)) - 1) kept[0] = run8 + (double)k * w8;
         }
-        const int left = top_k - (hit_count + n - c8);     // of this bin and later ones
-        const int last = __ffsll(__ballot(lane < 8 && left <= c8 && c8 > 0)) - 1;
-        Z = from_lane(run8 + (double)min(max(left, 0), c8) * w8, last < 0 ? 7 : last);
         __syncthreads();
+        Z = kept[0];
       }
     }
     // top-p: the shortest prefix that reaches p * Z
     if (top_p < 1.0) {
       const double goal = top_p * Z;
-      find([&](double sum) { return sum >= goal; });
-      const unsigned long long full = __ballot(lane < 8 && w8 > 0.0);
-      const unsigned long long over = __ballot(lane < 8 && w8 > 0.0 && run8 + (double)c8 * w8 >= goal);
-      const int e = over ? __ffsll(over) - 1 : 63 - __clzll(full);
-      const double n = fmin(fmax(ceil((goal - run8) / w8), 1.0), (double)c8);
-      Z = fmin(Z, from_lane(run8 + n * w8, e));
+      find(1, [&](double sum) { return sum >= goal; });
+      if (wave == 0) {
+        const unsigned long long full = __ballot(lane < 8 && w8 > 0.0);
+        const unsigned long long over = __ballot(lane < 8 && w8 > 0.0 && run8 + (double)c8 * w8 >= goal);
+        const double n = fmin(fmax(ceil((goal - run8) / w8), 1.0), (double)c8);
+        if (lane == (over ? __ffsll(over) - 1 : 63 - __clzll(full))) kept[1] = run8 + n * w8;
+      }
       __syncthreads();
+      Z = fmin(Z, kept[1]);
     }
     if (min_p > 0.0) {
-      const double s = wave_upto(mass_mp);
-      __syncthreads();                              // the running sums' ends have been read
-      if (lane == 63) ends_d[wave] = s;
-      __syncthreads();
       double mp = 0.0;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) mp += ends_d[w];
+      for (int w = 0; w < kWaves; ++w) mp += mp_d[w];
       Z = fmin(Z, min_p > 1.0 ? 1.0 : mp);
     }
     // the first token whose running sum exceeds u * Z
-    const double target = fmin(fmax((double)a.u[b], 0.0), 1.0 - 0x1p-24) * Z;
-    find([&](double sum) { return sum > target; });
-    const unsigned long long full = __ballot(lane < 8 && w8 > 0.0);
-    const unsigned long long over = __ballot(lane < 8 && w8 > 0.0 && run8 + (double)c8 * w8 > target);
-    const int e = over ? __ffsll(over) - 1 : 63 - __clzll(full);
-    bin = hit * kRun + e;
-    rank = (int)from_lane(fmin(fmax(floor((target - run8) / w8), 0.0), (double)(c8 - 1)), e);
-    const double w = from_lane(w8, e);
-    if (tid == 0) logp = log(w) - log(Z);
+    const double target = fmin(fmax((double)u, 0.0), 1.0 - 0x1p-24) * Z;
+    const int at = find(2, [&](double sum) { return sum > target; });
+    if (wave == 0) {
+      const unsigned long long full = __ballot(lane < 8 && w8 > 0.0);
+      const unsigned long long over = __ballot(lane < 8 && w8 > 0.0 && run8 + (double)c8 * w8 > target);
+      if (lane == (over ? __ffsll(over) - 1 : 63 - __clzll(full))) {
+        picked[0] = at * kRun + lane;
+        picked[1] = (int)fmin(fmax(floor((target - run8) / w8), 0.0), (double)(c8 - 1));
+        a.logprobs[b] = (float)(log(w8) - log(Z));
+      }
+    }
+    __syncthreads();
+    bin = picked[0];
+    rank = picked[1];
+  } else if (tid == 0) {
+    a.logprobs[b] = 0.f;
   }
-  if (tid == 0) a.logprobs[b] = (float)logp;
-  bin += top;
+  const int key = __builtin_amdgcn_readfirstlane(top - bin);
+  const unsigned key2 = ((unsigned)key & 0xFFFFu) * 0x10001u;
   // the rank-th token (by index) of that value
-  for (long long part = 0; part < span; part += kRound) {
-    if (!resident) x.load(row, a.V, part, skew, tid);
+  for (long long part = 0; part < (RESIDENT ? 1 : span); part += kRound) {
+    if (!RESIDENT) { x.load(row, part, left(part), skew, tid); x.to_keys(left(part)); }
+    typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
-      unsigned n = 0;
+      int n = 0;
+      if (c * kThreads * 8 < left(part)) {
+        u16x2 other = {0, 0};                       // halves that differ
 #pragma unroll
-      for (int e = 0; e < 8; ++e) n += __popcll(__ballot(x.place(c, e) == bin));
-      if (lane == 0) matches[c * kWaves + wave] = n;
+        for (int e = 0; e < 4; ++e) {
+          const unsigned w = x.r[c][e] ^ key2;
+          other += __builtin_elementwise_min(__builtin_bit_cast(u16x2, w), (u16x2){1, 1});
+        }
+        const int mine = 8 - (int)other[0] - (int)other[1];
+        if (__any(mine)) n = lane_of(wave_upto(mine), 63);
+      }
+      if (lane == 0) matches[c * kWaves + wave] = (unsigned)n;
     }
     __syncthreads();
     const u32x4 m4 = *reinterpret_cast<const u32x4*>(&matches[lane * 4]);
@@ -319,32 +362,33 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     const int end = wave_upto(mine), start = end - mine;
     const unsigned long long has = __ballot(rank >= start && rank < end);
     if (has) {
-      int where = lane * 4, left = rank - start;
+      int where = lane * 4, k = rank - start;
 #pragma unroll
       for (int q = 0; q < 3; ++q)
-        if (where == lane * 4 + q && left >= (int)m4[q]) { left -= (int)m4[q]; ++where; }
+        if (where == lane * 4 + q && k >= (int)m4[q]) { k -= (int)m4[q]; ++where; }
       const int owner = __ffsll(has) - 1;
-      where = from_lane(where, owner);
-      left = from_lane(left, owner);
+      where = lane_of(where, owner);
+      k = lane_of(k, owner);
       if (where % kWaves == wave) {
+        u32x4 y = x.r[0];
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c)
-          if (c == where / kWaves) {
-            int n = 0;
+        for (int c = 1; c < kChunks; ++c)
+          if (c == where / kWaves) y = x.r[c];
+        auto hit = [&](int e) { return ((y[e >> 1] ^ key2) & (e & 1 ? 0xFFFF0000u : 0xFFFFu)) == 0; };
+        int n = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) n += x.place(c, e) == bin;
-            const int ex = wave_upto(n) - n;
-            if (left >= ex && left < ex + n) {
-              int k = left - ex;
+        for (int e = 0; e < 8; ++e) n += hit(e);
+        const int ex = wave_upto(n) - n;
+        if (k >= ex && k < ex + n) {
+          int m = k - ex;
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                if (x.place(c, e) == bin && k-- == 0) a.tokens[b] = part + (long long)(c * kThreads + tid) * 8 - skew + e;
-            }
-          }
+          for (int e = 0; e < 8; ++e)
+            if (hit(e) && m-- == 0) a.tokens[b] = part + (long long)(where / kWaves * kThreads + tid) * 8 - skew + e;
+        }
       }
       return;
     }
-    rank -= from_lane(end, 63);
+    rank -= lane_of(end, 63);
     __syncthreads();
   }
 }
@@ -365,7 +409,7 @@ extern "C" int zk_sample(const void* logits, const float* u, const float* temper
   if (rows == 0) return ZK_OK;
   SampleArgs a{(const bf16_t*)logits, u, temperature_rows, top_p_rows, min_p_rows, top_k_rows, temperature, top_p, min_p,
                top_k, (long long*)tokens, logprobs, (long long)V, (long long)ld};
-  hipLaunchKernelGGL(sample_kernel, dim3((unsigned)rows), dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL(V + 7 <= kRound ? sample_kernel<true> : sample_kernel<false>, dim3((unsigned)rows), dim3(kThreads), 0, stream, a);
   ZK_CHECK_LAUNCH();
   return ZK_OK;
 }
