@@ -14,6 +14,10 @@ using namespace zkattn;
 namespace {
 
 constexpr float kLog2e = LOG2E;
+// The softmax is relative to a maximum that may lag the true one by this power of two: outputs and sums are rescaled only
+// when a score passes it (64 multiplies a piece otherwise), and neither fp32 sums nor bf16 probabilities lose anything to a
+// common factor of up to 2^8.
+constexpr float kSlack = 8.0f;
 
 // =========================================================================================
 // append: one workgroup per token, a unit of work is 16 values of a head (two 16-byte chunks) that turn by 8 angles.
@@ -98,30 +102,32 @@ struct PagedArgs {
   float scale;
 };
 
+constexpr int kMaxRows = 1 << 30;
+
 // one sequence's share of the call
 struct Seq {
   int q0, n, len;               // first row of q, new tokens, cached rows
-  long long first;              // cached rows before the new tokens (as the lengths say: negative if they do not fit)
+  int first;                    // cached rows before the new tokens (as the lengths say: negative if they do not fit)
   __device__ __forceinline__ Seq(const PagedArgs& a, int b) {
     q0 = min(max(a.cu[b], 0), a.T);
     n = min(max(a.cu[b + 1], q0), a.T) - q0;
-    len = (int)min((long long)max(a.ctx[b], 0), (long long)a.table_cols * a.page_size);
-    first = (long long)a.ctx[b] - n;
+    const int c = min(max(a.ctx[b], 0), kMaxRows);  // and T < kMaxRows: differences of the two fit 32 bits
+    len = (int)min((long long)c, (long long)a.table_cols * a.page_size);
+    first = c - n;
   }
 };
 
 // which of the 32 keys from `base` on new token i (row q0 + i of q) may see, as bits; the cache's end is not looked at
-__device__ __forceinline__ unsigned seen_bits(const PagedArgs& a, const Seq& s, int i, long long base) {
-  const long long j0 = base - s.first;              // key `base` is new token j0 (negative: a row before them)
-  if (j0 + 32 <= 0) return ~0u;
+__device__ __forceinline__ unsigned seen_bits(const PagedArgs& a, const Seq& s, int i, int base) {
+  const int j0 = base - s.first;                    // key `base` is new token j0 (negative: a row before them)
   if (!a.mask) {                                    // keys up to the token's own
-    const long long c = i - j0 + 1;
-    return c >= 32 ? ~0u : c <= 0 ? 0u : (1u << (int)c) - 1u;
+    const int c = i - j0 + 1;
+    return c >= 32 ? ~0u : c <= 0 ? 0u : (1u << c) - 1u;
   }
+  if (j0 <= -32) return ~0u;
   const unsigned long long* m = a.mask + (size_t)(s.q0 + i) * a.mask_words;
-  if (j0 < 0) return (unsigned)(m[0] << (int)-j0) | ((1u << (int)-j0) - 1u);
-  const long long w = j0 >> 6;
-  const int sh = (int)(j0 & 63);
+  if (j0 < 0) return (unsigned)(m[0] << -j0) | ((1u << -j0) - 1u);
+  const int w = j0 >> 6, sh = j0 & 63;
   unsigned long long x = w < a.mask_words ? m[w] >> sh : 0ull;
   if (sh > 32 && w + 1 < a.mask_words) x |= m[w + 1] << (64 - sh);
   return (unsigned)x;
@@ -135,18 +141,20 @@ __device__ __forceinline__ int cache_row(const PagedArgs& a, int b, int key, int
   return pg < (unsigned)a.n_pages ? (int)(pg * (unsigned)a.page_size + ((unsigned)key - at * (unsigned)a.page_size)) : -1;
 }
 
-// workgroup -> (sequence, kv head, share, row tile), tiles fastest; an XCD (workgroups id % 8) takes consecutive work, so
-// that the tiles that read the same keys find them in its L2
+// workgroup -> (sequence, share, kv head, row tile).  Row tiles of one (sequence, share, kv head) read the same keys: they
+// are neighbours on one XCD (workgroups of equal id % 8), so that its L2 serves all but the first; these groups are dealt to
+// the XCDs in turn, so that long sequences load all of them.
 struct Work {
   int tile, split, kvh, b;
   bool any;
   __device__ __forceinline__ Work(const PagedArgs& a) {
-    int w = (int)(blockIdx.x & 7) * ((a.groups + 7) >> 3) + (int)(blockIdx.x >> 3);
-    any = w < a.groups && (int)(blockIdx.x >> 3) < ((a.groups + 7) >> 3);
-    tile = w % a.tiles; w /= a.tiles;
-    split = w % a.splits; w /= a.splits;
-    kvh = w % a.Hkv;
-    b = w / a.Hkv;
+    int w = (int)(blockIdx.x >> 3);
+    tile = w % a.tiles;
+    w = w / a.tiles * 8 + (int)(blockIdx.x & 7);
+    any = w < a.groups;
+    kvh = w % a.Hkv; w /= a.Hkv;
+    split = w % a.splits;
+    b = w / a.splits;
   }
 };
 
@@ -253,16 +261,18 @@ __global__ __launch_bounds__(256, MT == 1 ? (HD == 128 ? 3 : 4) : 2) void attn_p
       for (int e = 1; e < 8; ++e) mx = fmaxf(mx, sc4[mt][e >> 2][e & 3]);
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float mn = fmaxf(m[mt], mx * sc);
-      const float use = mn == -INFINITY ? 0.f : mn;
-      const float f = __builtin_amdgcn_exp2f(m[mt] - use);
-      l[mt] *= f;
+      mx *= sc;
+      if (__any(mx > m[mt] + kSlack)) {
+        const float mn = fmaxf(m[mt], mx), f = fast_exp2(m[mt] - (mn == -INFINITY ? 0.f : mn));
+        l[mt] *= f;
 #pragma unroll
-      for (int d = 0; d < DB; ++d) o[mt][d] *= f;
-      m[mt] = mn;
+        for (int d = 0; d < DB; ++d) o[mt][d] *= f;
+        m[mt] = mn;
+      }
+      const float use = m[mt] == -INFINITY ? 0.f : m[mt];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc4[mt][e >> 2][e & 3], sc, -use));
+        const float x = fast_exp2(__builtin_fmaf(sc4[mt][e >> 2][e & 3], sc, -use));
         l[mt] += x;
         p[mt][e] = (__bf16)x;                       // rounded to bf16 for the matrix product only
       }
@@ -281,8 +291,7 @@ __global__ __launch_bounds__(256, MT == 1 ? (HD == 128 ? 3 : 4) : 2) void attn_p
   };
 
   // pieces that every row of the tile sees whole: up to the tile's first token in a chain, to the new tokens in a tree
-  const long long clear = s.first + (a.mask ? 0 : r0 / G + 1);
-  const int bulk = (int)min((long long)ke, max(clear, 0ll));
+  const int bulk = min(ke, s.first + (a.mask ? 0 : r0 / G + 1));
   int base = ks + 32 * wave;
   if (base + 32 <= bulk) {
     int row = cache_row(a, b, base + (lane & 31), bulk);
@@ -370,7 +379,7 @@ __global__ __launch_bounds__(256, MT == 1 ? (HD == 128 ? 3 : 4) : 2) void attn_p
     {
       const int r = mt * 16 + col;
       const float M = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
-      const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[mt] - M);
+      const float f = M == -INFINITY ? 0.f : fast_exp2(m[mt] - M);
 #pragma unroll
       for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4*>(xo + (wave * 16 + col) * LDO + d * 16 + 4 * g4) = o[mt][d] * f;
     }
@@ -381,7 +390,7 @@ __global__ __launch_bounds__(256, MT == 1 ? (HD == 128 ? 3 : 4) : 2) void attn_p
       const float M = fmaxf(fmaxf(sm[0][lr], sm[1][lr]), fmaxf(sm[2][lr], sm[3][lr]));
       float L = 0.f, y[per];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) L += M == -INFINITY ? 0.f : sl[w][lr] * __builtin_amdgcn_exp2f(sm[w][lr] - M);
+      for (int w = 0; w < 4; ++w) L += M == -INFINITY ? 0.f : sl[w][lr] * fast_exp2(sm[w][lr] - M);
 #pragma unroll
       for (int e = 0; e < per; ++e)
         y[e] = (xo[orow * LDO + oc + e] + xo[(16 + orow) * LDO + oc + e]) +
@@ -412,11 +421,14 @@ __global__ __launch_bounds__(256, MT == 1 ? (HD == 128 ? 3 : 4) : 2) void attn_p
 // chunk-swizzled, two stages, one barrier per tile; S^T = K Q^T and O^T += V^T P^T in 32x32x16 MFMAs with the row on
 // the lane, as in zk_attn_fwd.  Bound by the matrix and vector pipes in turn; see that kernel's header.
 // =========================================================================================
-template <int HD>
+// ONE_PAGE: page_size is a multiple of 64, so a tile lies in one page: its address is uniform and a lane's offset into it
+// constant, where pages of any size cost a look-up, four exchanges and 64-bit multiplies a lane and tile.
+template <int HD, bool ONE_PAGE>
 __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedArgs a) {
   using C = Cfg<HD>;
   constexpr int KV = 64, RB = HD * 2, TB = KV * RB, STAGE = 2 * TB, CPR = HD / 8, NQ = KV * CPR / 256;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * STAGE];
+  __shared__ unsigned bad[2];
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Work w(a);
@@ -430,31 +442,34 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedArgs a) {
   const bool alone = ks == 0 && ke == s.len;
   const float sc = a.scale * kLog2e;
   const int r0 = t0 + wave * 32, r = r0 + (lane & 31), rc = min(r, rows - 1), tok = rc / G;
-  // keys that the workgroup / this wave needs at all
-  const long long last_wg = a.mask ? s.len : s.first + min(t0 + 127, rows - 1) / G + 1;
-  const long long last_wave = r0 >= rows ? 0 : a.mask ? s.len : s.first + min(r0 + 31, rows - 1) / G + 1;
-  const int end = (int)min((long long)ke, max(last_wg, (long long)ks));
-  const int nt = (end - ks + KV - 1) / KV;
+  // keys that the workgroup / this wave needs at all, and those that every row of the workgroup sees
+  const int last_wg = a.mask ? s.len : s.first + min(t0 + 127, rows - 1) / G + 1;
+  const int last_wave = r0 >= rows ? 0 : a.mask ? s.len : s.first + min(r0 + 31, rows - 1) / G + 1;
+  const int clear = min(ke, s.first + (a.mask ? 0 : t0 / G + 1));
+  const int nt = (min(ke, max(last_wg, ks)) - ks + KV - 1) / KV;
   const bf16_t* kb = a.k + kvh * HD;
   const bf16_t* vb = a.v + kvh * HD;
 
-  auto issue = [&](int t, int rr) __attribute__((always_inline)) {         // rr: cache row of key `lane` of tile t
+  int row, next = -1;                               // cache row of key `lane` (ONE_PAGE: of the first key) of a tile
+  auto look = [&](int t) __attribute__((always_inline)) { return cache_row(a, b, ks + t * KV + (ONE_PAGE ? 0 : lane), ke); };
+  auto issue = [&](int t, int rr) __attribute__((always_inline)) {
     unsigned char* st = smem + (t & 1) * STAGE;
+    const size_t tile0 = ONE_PAGE ? (size_t)max(__builtin_amdgcn_readfirstlane(rr), 0) * kvw : 0;
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
       const int sidx = tid + 256 * i, trow = sidx / CPR, ch = (sidx % CPR) ^ swz_key<HD>(trow);
-      const size_t off = (size_t)max(__shfl(rr, trow, 64), 0) * kvw + ch * 8;
+      const size_t off = ONE_PAGE ? (size_t)(unsigned)(trow * kvw + ch * 8) : (size_t)max(__shfl(rr, trow, 64), 0) * kvw + ch * 8;
       unsigned char* dst = st + (wave * 64 + 256 * i) * 16;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kb + off),
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kb + tile0 + off),
                                        (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vb + off),
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vb + tile0 + off),
                                        (__attribute__((address_space(3))) void*)(dst + TB), 16, 0, 0);
     }
   };
-  int row = cache_row(a, b, ks + lane, ke), next = -1;
+  row = look(0);
   if (nt > 0) {
     issue(0, row);
-    next = cache_row(a, b, ks + KV + lane, ke);
+    next = look(1);
   }
   bf16x8 qf[C::DS];
   {
@@ -471,124 +486,119 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedArgs a) {
 #pragma unroll
   for (int ds = 0; ds < C::DS; ++ds) asm volatile("" ::"v"(qf[ds]));
 
-  f32x16 st[2];
-  int t = 0;
-  const unsigned char *kl, *vl;
-  auto landed = [&]() __attribute__((always_inline)) {           // tile t is here, tile t - 1 is consumed: its stage takes t + 1
+  for (int t = 0; t < nt; ++t) {
+    const int k0 = ks + t * KV;
+    unsigned long long ok;                          // keys of the tile that exist; the same in every wave
+    if (ONE_PAGE) ok = __builtin_amdgcn_readfirstlane(row) < 0 ? 0ull : ke - k0 >= 64 ? ~0ull : (1ull << (ke - k0)) - 1;
+    else ok = __ballot(row >= 0);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    kl = smem + (t & 1) * STAGE;
-    vl = kl + TB;
+    __syncthreads();                                // tile t is here, tile t - 1 is consumed: its stage takes t + 1
+    unsigned char* kl = smem + (t & 1) * STAGE;
+    unsigned char* vl = kl + TB;
     row = next;
     if (t + 1 < nt) {
       issue(t + 1, row);
-      next = cache_row(a, b, ks + (t + 2) * KV + lane, ke);
+      next = look(t + 2);
     }
-  };
-  auto scores = [&]() __attribute__((always_inline)) {
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) st[x][e] = 0.f;
-#pragma unroll
-      for (int ds = 0; ds < C::DS; ++ds)
-        st[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag_sw<HD>(kl, x * 32, ds, lane), qf[ds], st[x], 0, 0, 0);
-    }
-  };
-  auto softmax = [&]() __attribute__((always_inline)) {
-    float mx = fmaxf(st[0][0], st[1][0]);
-#pragma unroll
-    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, fmaxf(st[0][e], st[1][e]));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float mn = fmaxf(m_run, mx * sc);
-    const float use = mn == -INFINITY ? 0.f : mn;
-    const float f = fast_exp2(m_run - use);
-    float rs = 0.f;
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float p = fast_exp2(__builtin_fmaf(st[x][e], sc, -use));
-        st[x][e] = p;
-        rs += p;
-      }
-    l_run = l_run * f + rs;
-    m_run = mn;
-#pragma unroll
-    for (int d = 0; d < C::DB; ++d) o[d] = o[d] * f;
-  };
-  auto product = [&]() __attribute__((always_inline)) {
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int z = 0; z < 2; ++z) {
-        const bf16x8 pf = pack_acc(st[x], z);
-#pragma unroll
-        for (int d = 0; d < C::DB; ++d)
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_frag_sw<HD>(vl, x * 32, z, d, lane), pf, o[d], 0, 0, 0);
-      }
-  };
-  // tiles that every row of the workgroup sees whole
-  const long long clear_wg = min((long long)ke, s.first + (a.mask ? 0 : t0 / G + 1)) - ks;
-  const int bulk = clear_wg < KV ? 0 : (int)(clear_wg / KV);
-  while (t < bulk && __all(row >= 0)) {
-    landed();
-    scores();
-    softmax();
-    product();
-    ++t;
-  }
-  // the others: the cache's end, new tokens, pages that do not exist (and what stands behind one)
-  for (; t < nt; ++t) {
-    const int k0 = ks + t * KV;
-    const unsigned long long ok = __ballot(row >= 0);           // the same in every wave
-    landed();
-    // rows that do not exist are zeros in V (their p is 0, and 0 x NaN is not); infinities and NaN are looked for
-    bool odd = false;
-#pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-      const int sidx = tid + 256 * i;
-      u32x4* x = reinterpret_cast<u32x4*>(const_cast<unsigned char*>(vl) + sidx * 16);
-      if (!((ok >> (sidx / CPR)) & 1)) *x = u32x4{0u, 0u, 0u, 0u};
-      else {
-        const u32x4 y = *x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) odd |= not_finite(y[e]);
-      }
-    }
-    const bool any_odd = __syncthreads_or((int)odd) != 0;
-    if (k0 >= last_wave) continue;
-    scores();
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const unsigned vis = seen_bits(a, s, tok, k0 + 32 * x) & (unsigned)(ok >> (32 * x));
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (!((vis >> acc_row(e, h)) & 1)) st[x][e] = -INFINITY;
-    }
-    softmax();
-    if (!any_odd) {
-      product();
-    } else {
-      // key by key, keys with p = 0 passed over
+    const bool edge = k0 + KV > clear || ok != ~0ull;        // uniform over the workgroup: some row may not see some key
+    unsigned long long odd = 0;
+    if (__builtin_expect(edge, 0)) {
+      // V rows that do not exist become zeros (their p is 0, and 0 x NaN is not); rows with infinities or NaN are noted
+      if (tid < 2) bad[tid] = 0;
+      __syncthreads();
 #pragma unroll 1
-      for (int kk = 0; kk < KV; ++kk) {
-        float x = 0.f;
-#pragma unroll
-        for (int e = 0; e < 32; ++e)
-          if (e == (kk >> 5) * 16 + (kk & 3) + 4 * ((kk & 31) >> 3)) x = st[e >> 4][e & 15];
-        x = (float)(__bf16)__shfl(x, ((kk >> 2) & 1) * 32 + (lane & 31), 64);
-        if (x == 0.f) continue;
-#pragma unroll
-        for (int d = 0; d < C::DB; ++d)
-#pragma unroll
-          for (int r4 = 0; r4 < 4; ++r4) {
-            const int ch = d * 4 + r4;
-            const u32x2 y = *reinterpret_cast<const u32x2*>(vl + kk * RB + ((ch ^ swz_key<HD>(kk)) << 4) + 8 * h);
-            o[d][4 * r4] += x * lo_bf(y[0]); o[d][4 * r4 + 1] += x * hi_bf(y[0]);
-            o[d][4 * r4 + 2] += x * lo_bf(y[1]); o[d][4 * r4 + 3] += x * hi_bf(y[1]);
-          }
+      for (int i = 0; i < NQ; ++i) {
+        const int sidx = tid + 256 * i, trow = sidx / CPR;
+        u32x4* x = reinterpret_cast<u32x4*>(vl + sidx * 16);
+        const u32x4 y = *x;
+        if (!((ok >> trow) & 1)) *x = u32x4{0u, 0u, 0u, 0u};
+        else if (not_finite(y[0]) || not_finite(y[1]) || not_finite(y[2]) || not_finite(y[3])) atomicOr(&bad[trow >> 5], 1u << (trow & 31));
       }
+      __syncthreads();
+      odd = ((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)bad[1]) << 32) |
+            (unsigned)__builtin_amdgcn_readfirstlane((int)bad[0]);
+    }
+    f32x16 st[2];
+    const bool wanted = k0 < last_wave;
+    if (wanted) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) st[x][e] = 0.f;
+#pragma unroll
+        for (int ds = 0; ds < C::DS; ++ds)
+          st[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag_sw<HD>(kl, x * 32, ds, lane), qf[ds], st[x], 0, 0, 0);
+      }
+      if (__builtin_expect(edge, 0)) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const unsigned vis = seen_bits(a, s, tok, k0 + 32 * x) & (unsigned)(ok >> (32 * x));
+#pragma unroll
+          for (int e = 0; e < 16; ++e) st[x][e] = (vis >> acc_row(e, h)) & 1 ? st[x][e] : -INFINITY;
+        }
+      }
+      float mx = fmaxf(st[0][0], st[1][0]);
+#pragma unroll
+      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, fmaxf(st[0][e], st[1][e]));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * sc;
+      if (__any(mx > m_run + kSlack)) {
+        const float mn = fmaxf(m_run, mx), f = fast_exp2(m_run - (mn == -INFINITY ? 0.f : mn));
+        l_run *= f;
+        m_run = mn;
+#pragma unroll
+        for (int d = 0; d < C::DB; ++d) o[d] = o[d] * f;
+      }
+      const float use = m_run == -INFINITY ? 0.f : m_run;
+      float rs = 0.f;
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float p = fast_exp2(__builtin_fmaf(st[x][e], sc, -use));
+          st[x][e] = p;
+          rs += p;
+        }
+      l_run += rs;
+    }
+    if (__builtin_expect(odd != 0, 0)) {
+      // keys with infinities or NaN in V: added on their own to the rows that see them, then zeros for the product below
+      if (wanted) {
+#pragma unroll 1
+        for (unsigned long long left = odd; left; left &= left - 1) {
+          const int kk = __ffsll(left) - 1;
+          float x = 0.f;
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (e == (kk >> 5) * 16 + (kk & 3) + 4 * ((kk & 31) >> 3)) x = st[e >> 4][e & 15];
+          x = __shfl(x, ((kk >> 2) & 1) * 32 + (lane & 31), 64);
+          if (x != 0.f) {
+#pragma unroll
+            for (int d = 0; d < C::DB; ++d)
+#pragma unroll
+              for (int r4 = 0; r4 < 4; ++r4) {
+                const u32x2 y = *reinterpret_cast<const u32x2*>(vl + kk * RB + (((d * 4 + r4) ^ swz_key<HD>(kk)) << 4) + 8 * h);
+                o[d][4 * r4] += x * lo_bf(y[0]); o[d][4 * r4 + 1] += x * hi_bf(y[0]);
+                o[d][4 * r4 + 2] += x * lo_bf(y[1]); o[d][4 * r4 + 3] += x * hi_bf(y[1]);
+              }
+          }
+        }
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int i = 0; i < NQ; ++i)
+        if ((odd >> ((tid + 256 * i) / CPR)) & 1) *reinterpret_cast<u32x4*>(vl + (tid + 256 * i) * 16) = u32x4{0u, 0u, 0u, 0u};
+      __syncthreads();
+    }
+    if (wanted) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const bf16x8 pf = pack_acc(st[x], z);
+#pragma unroll
+          for (int d = 0; d < C::DB; ++d)
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_frag_sw<HD>(vl, x * 32, z, d, lane), pf, o[d], 0, 0, 0);
+        }
     }
   }
   const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
@@ -740,7 +750,7 @@ extern "C" int zk_attn_paged(const void* q, const void* k_cache, const void* v_c
   const int rc = zk_attn_paged_ws(B, T, max_q, max_ctx, Hq, Hkv, head_dim, &need);
   if (rc != ZK_OK) return rc;
   if (page_size <= 0 || n_pages <= 0 || table_cols <= 0 || ld_table < table_cols) return ZK_EINVAL;
-  if (T > 0x7FFFFFFF || B > 0x7FFFFFFE || page_size > 0x7FFFFFFF || n_pages > 0x7FFFFFFF || ld_table > 0x7FFFFFFF) return ZK_EINVAL;
+  if (T >= kMaxRows || B > 0x7FFFFFFE || page_size > 0x7FFFFFFF || n_pages > 0x7FFFFFFF || ld_table > 0x7FFFFFFF) return ZK_EINVAL;
   if (n_pages * page_size > 0x7FFFFFFF || T * Hq > 0x7FFFFFFF || Hkv * head_dim > (1 << 24)) return ZK_EINVAL;
   if ((ldq & 7) || (ldo & 7) || ldq < Hq * head_dim || ldo < Hq * head_dim) return ZK_EINVAL;
   if (!q || !k_cache || !v_cache || !out || !page_table || !ctx_lens || !cu_q) return ZK_EINVAL;
@@ -749,8 +759,8 @@ extern "C" int zk_attn_paged(const void* q, const void* k_cache, const void* v_c
     return ZK_EINVAL;
   if (T == 0) return ZK_OK;
   const Plan p = plan_of(B, max_q, max_ctx, Hq, Hkv);
-  const int64_t groups = B * Hkv * p.tiles * p.splits;
-  if (groups > 0x7FFFFFF0) return ZK_EINVAL;
+  const int64_t groups = B * Hkv * p.splits;         // each of p.tiles workgroups
+  if ((groups + 7) * p.tiles > 0x7FFFFFF0) return ZK_EINVAL;
   int lg = 0;                                       // page_mul: the 31-bit reciprocal, rounded up (exact below 2^31)
   while ((int64_t)1 << lg < page_size) ++lg;
   const unsigned mul = (unsigned)((((unsigned long long)1 << (31 + lg)) / (unsigned long long)page_size) + 1);
@@ -759,10 +769,11 @@ extern "C" int zk_attn_paged(const void* q, const void* k_cache, const void* v_c
               (const unsigned long long*)tree_mask, part_o, part_o ? ws + T * Hq * p.splits * head_dim : nullptr, (int)T,
               (int)B, (int)Hq, (int)Hkv, (int)page_size, (int)n_pages, (int)table_cols, (int)ld_table, (int)mask_words,
               p.tiles, p.splits, p.split_keys, (int)groups, mul, (unsigned)(31 + lg), (long long)ldq, (long long)ldo, scale};
+  const bool one_page = page_size % 64 == 0;
   void (*kern)(PagedArgs) =
-      head_dim == 128 ? (p.mt == 1 ? attn_paged_stream_kernel<128, 1> : p.mt == 2 ? attn_paged_stream_kernel<128, 2> : attn_paged_tile_kernel<128>)
-                      : (p.mt == 1 ? attn_paged_stream_kernel<64, 1> : p.mt == 2 ? attn_paged_stream_kernel<64, 2> : attn_paged_tile_kernel<64>);
-  hipLaunchKernelGGL(kern, dim3((unsigned)((groups + 7) / 8 * 8)), dim3(256), 0, stream, a);
+      head_dim == 128 ? (p.mt == 1 ? attn_paged_stream_kernel<128, 1> : p.mt == 2 ? attn_paged_stream_kernel<128, 2> : one_page ? attn_paged_tile_kernel<128, true> : attn_paged_tile_kernel<128, false>)
+                      : (p.mt == 1 ? attn_paged_stream_kernel<64, 1> : p.mt == 2 ? attn_paged_stream_kernel<64, 2> : one_page ? attn_paged_tile_kernel<64, true> : attn_paged_tile_kernel<64, false>);
+  hipLaunchKernelGGL(kern, dim3((unsigned)((groups + 7) / 8 * 8 * p.tiles)), dim3(256), 0, stream, a);
   if (p.splits > 1) {
     void (*merge)(PagedArgs) = head_dim == 128 ? attn_paged_merge_kernel<128> : attn_paged_merge_kernel<64>;
     hipLaunchKernelGGL(merge, dim3((unsigned)(T * Hq)), dim3((unsigned)head_dim), 0, stream, a);
