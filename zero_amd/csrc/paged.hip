@@ -421,6 +421,18 @@ __global__ __launch_bounds__(256, MT == 1 ? (HD == 128 ? 3 : 4) : 2) void attn_p
 // chunk-swizzled, two stages, one barrier per tile; S^T = K Q^T and O^T += V^T P^T in 32x32x16 MFMAs with the row on
 // the lane, as in zk_attn_fwd.  Bound by the matrix and vector pipes in turn; see that kernel's header.
 // =========================================================================================
+// LDS-DMA of 16 bytes a lane to consecutive LDS from the wave-uniform `dst` on; sources per lane, or a uniform base and a
+// 32-bit byte offset.  Inline asm, not the builtin: behind a builtin the compiler waits for every DMA in flight before the
+// first transposed LDS read, whatever tile that reads, and so for tile t + 1 in the middle of tile t.  The loop waits by
+// hand (vmcnt(0) and a barrier before a tile's first read); no register is written, m0 is used by nothing else here.
+__device__ __forceinline__ void lds_dma_from(const void* dst, const void* src) {
+  const unsigned m = __builtin_amdgcn_readfirstlane((unsigned)(unsigned long)(__attribute__((address_space(3))) void*)const_cast<void*>(dst));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m), "v"(src) : "memory");
+}
+__device__ __forceinline__ void lds_dma_at(const void* dst, const void* base, unsigned off) {
+  const unsigned m = __builtin_amdgcn_readfirstlane((unsigned)(unsigned long)(__attribute__((address_space(3))) void*)const_cast<void*>(dst));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m), "v"(off), "s"(base) : "memory");
+}
 // ONE_PAGE: page_size is a multiple of 64, so a tile lies in one page: its address is uniform and a lane's offset into it
 // constant, where pages of any size cost a look-up, four exchanges and 64-bit multiplies a lane and tile.
 template <int HD, bool ONE_PAGE>
@@ -460,10 +472,13 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedArgs a) {
       const int sidx = tid + 256 * i, trow = sidx / CPR, ch = (sidx % CPR) ^ swz_key<HD>(trow);
       const size_t off = ONE_PAGE ? (size_t)(unsigned)(trow * kvw + ch * 8) : (size_t)max(__shfl(rr, trow, 64), 0) * kvw + ch * 8;
       unsigned char* dst = st + (wave * 64 + 256 * i) * 16;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kb + tile0 + off),
-                                       (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vb + tile0 + off),
-                                       (__attribute__((address_space(3))) void*)(dst + TB), 16, 0, 0);
+      if (ONE_PAGE) {
+        lds_dma_at(dst, kb + tile0, (unsigned)(off * 2));
+        lds_dma_at(dst + TB, vb + tile0, (unsigned)(off * 2));
+      } else {
+        lds_dma_from(dst, kb + off);
+        lds_dma_from(dst + TB, vb + off);
+      }
     }
   };
   row = look(0);
