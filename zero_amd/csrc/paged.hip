@@ -117,6 +117,17 @@ struct Seq {
   }
 };
 
+// the last sequence that starts at or before row t of q
+__device__ __forceinline__ int seq_of(const PagedArgs& a, int t) {
+  if (t < a.B && a.cu[t] == t && a.cu[t + 1] == t + 1) return t;      // single tokens
+  int lo = 0, hi = a.B;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.cu[mid] <= t) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
 // which of the 32 keys from `base` on new token i (row q0 + i of q) may see, as bits; the cache's end is not looked at
 __device__ __forceinline__ unsigned seen_bits(const PagedArgs& a, const Seq& s, int i, int base) {
   const int j0 = base - s.first;                    // key `base` is new token j0 (negative: a row before them)
@@ -178,7 +189,7 @@ struct Merge {
 };
 
 template <int HD, int MT>
-__global__ __launch_bounds__(256, MT == 1 ? (HD == 128 ? 3 : 4) : 2) void attn_paged_stream_kernel(PagedArgs a) {
+__global__ __launch_bounds__(256, MT == 1 && HD == 64 ? 4 : 2) void attn_paged_stream_kernel(PagedArgs a) {
   constexpr int CPR = HD / 8, KC = HD / 32, DB = HD / 16, NV = HD / 16, LDO = Merge<HD>::LDO;
   constexpr int VB = 32 * HD * 2;                   // one wave's V piece
   constexpr int XB = 4 * 16 * LDO * 4;
@@ -644,59 +655,90 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedArgs a) {
 }
 
 // out = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the shares of a row's sequence, in a fixed order: one workgroup
-// per (token, head), four groups of HD / 4 threads take every fourth share and are added in order
-template <int HD>
-__global__ __launch_bounds__(HD) void attn_paged_merge_kernel(PagedArgs a) {
-  constexpr int TPG = HD / 4, NG = 4;
+// per (token, head, slice of COLS columns); COLS / 4 threads read a share's columns, the others every following share, and
+// the groups' sums are added in order.
+constexpr int kMergeThreads = 256;
+template <int HD, int COLS>
+__global__ __launch_bounds__(kMergeThreads) void attn_paged_merge_kernel(PagedArgs a) {
+  constexpr int TPG = COLS / 4, NG = kMergeThreads / TPG, NSL = HD / COLS;
   __shared__ float wgt[1024];
-  __shared__ __attribute__((aligned(16))) float acc[NG][HD];
-  __shared__ float red[4];
-  const int t = blockIdx.x / a.Hq, h = blockIdx.x % a.Hq, d = threadIdx.x;
-  int lo = 0, hi = a.B;                             // last sequence that starts at or before row t
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu[mid] <= t) lo = mid; else hi = mid;
-  }
-  const Seq s(a, lo);
+  __shared__ __attribute__((aligned(16))) float acc[NG][COLS];
+  __shared__ float red[4], sum[4];
+  const int id = blockIdx.x / NSL, t = id / a.Hq, h = id % a.Hq, col0 = blockIdx.x % NSL * COLS, tid = threadIdx.x;
+  const Seq s(a, seq_of(a, t));
   if (t < s.q0 || t >= s.q0 + s.n) return;
   const int parts = min(a.splits, (s.len + a.split_keys - 1) / a.split_keys);
   if (parts <= 1) return;                           // written by its only share
-  const float* ml = a.part_ml + (size_t)blockIdx.x * a.splits * 2;
-  const float* po = a.part_o + (size_t)blockIdx.x * a.splits * HD;
+  const float* ml = a.part_ml + (size_t)id * a.splits * 2;
+  const float* po = a.part_o + (size_t)id * a.splits * HD + col0;
   float M = -INFINITY;
-  for (int i = d; i < parts; i += HD) M = fmaxf(M, ml[2 * i]);
+  for (int i = tid; i < parts; i += kMergeThreads) M = fmaxf(M, ml[2 * i]);
   M = wave_max(M);
-  if ((d & 63) == 0) red[d >> 6] = M;
+  if ((tid & 63) == 0) red[tid >> 6] = M;
   __syncthreads();
-  for (int i = 0; i < HD / 64; ++i) M = fmaxf(M, red[i]);
-  const int g = d / TPG, c = (d % TPG) * 4;
+  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const int g = tid / TPG, c = (tid % TPG) * 4;
   f32x4 y = {0.f, 0.f, 0.f, 0.f};
   float L = 0.f;
   for (int i0 = 0; i0 < parts; i0 += 1024) {
     const int np = min(1024, parts - i0);
     __syncthreads();
-    for (int i = d; i < np; i += HD) {
+    for (int i = tid; i < np; i += kMergeThreads) {
       const float f = M == -INFINITY ? 0.f : fast_exp2(ml[2 * (i0 + i)] - M);
       wgt[i] = f;
       L += ml[2 * (i0 + i) + 1] * f;
     }
     __syncthreads();
 #pragma unroll 4
-    for (int i = g; i < np; i += NG) {
-      // a share that saw nothing of this row has weight 0 and an output of zeros
+    for (int i = g; i < np; i += NG) {              // (a share that saw nothing of this row has weight 0 and zeros)
       const f32x4 x = *reinterpret_cast<const f32x4*>(po + (size_t)(i0 + i) * HD + c);
       y += x * wgt[i];
     }
   }
   *reinterpret_cast<f32x4*>(&acc[g][c]) = y;
   L = wave_sum(L);
+  if ((tid & 63) == 0) sum[tid >> 6] = L;
   __syncthreads();
-  if ((d & 63) == 0) red[d >> 6] = L;
-  __syncthreads();
-  L = 0.f;
-  for (int i = 0; i < HD / 64; ++i) L += red[i];
+  if (tid >= COLS) return;
+  L = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  float v = 0.f;
+#pragma unroll
+  for (int i = 0; i < NG; ++i) v += acc[i][tid];
   const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
-  a.out[(size_t)t * a.ldo + (size_t)h * HD + d] = f2bf(((acc[0][d] + acc[1][d]) + (acc[2][d] + acc[3][d])) * inv);
+  a.out[(size_t)t * a.ldo + (size_t)h * HD + col0 + tid] = f2bf(v * inv);
+}
+
+// the same for few shares: a wave a row, HD / 64 columns a lane, four rows a workgroup
+template <int HD>
+__global__ __launch_bounds__(256) void attn_paged_merge_few_kernel(PagedArgs a) {
+  constexpr int CPL = HD / 64;
+  const int lane = threadIdx.x & 63;
+  const int id = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+  if (id >= a.T * a.Hq) return;
+  const int t = id / a.Hq, h = id % a.Hq;
+  const Seq s(a, seq_of(a, t));
+  if (t < s.q0 || t >= s.q0 + s.n) return;
+  const int parts = min(a.splits, (s.len + a.split_keys - 1) / a.split_keys);
+  if (parts <= 1) return;
+  const float* ml = a.part_ml + (size_t)id * a.splits * 2;
+  const float* po = a.part_o + (size_t)id * a.splits * HD + lane * CPL;
+  float m = lane < parts ? ml[2 * lane] : -INFINITY, l = lane < parts ? ml[2 * lane + 1] : 0.f;
+  const float M = wave_max(m);
+  const float f = M == -INFINITY ? 0.f : fast_exp2(m - M);
+  const float L = wave_sum(l * f);
+  const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
+  float y[CPL];
+#pragma unroll
+  for (int c = 0; c < CPL; ++c) y[c] = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) {
+    const float w = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(f), i));
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) y[c] += po[(size_t)i * HD + c] * w;
+  }
+  bf16_t* op = a.out + (size_t)t * a.ldo + (size_t)h * HD + lane * CPL;
+  if (CPL == 2) *reinterpret_cast<unsigned*>(op) = pack2bf(y[0] * inv, y[CPL - 1] * inv);
+  else *op = f2bf(y[0] * inv);
 }
 
 // shape of a launch: host arithmetic on the sizes alone
@@ -708,14 +750,16 @@ inline Plan plan_of(int64_t B, int64_t max_q, int64_t max_ctx, int64_t Hq, int64
   const int64_t rows = max_q * (Hq / Hkv);
   p.mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 8;
   p.tiles = (int)((rows + 16 * p.mt - 1) / (16 * p.mt));
-  // shares of the keys: enough workgroups for two rounds of what the 256 CUs hold at two a CU, none under 128 keys (one
-  // piece a wave), and none over 2048 while there are fewer groups than that
+  // shares of the keys: as many as fill the 512 workgroups that the CUs hold at two each, none under 128 keys (a piece for
+  // each wave).  The stream kernel's shares end at 512 keys: the lengths of a batch differ, and small shares even that out
+  // (48 sequences of 700 to 8192: 150 us with 1024 keys, 140 with 512).  The tile kernel's do not: a share costs it a
+  // prologue of several tiles and 130 floats a row through memory.
   const int64_t groups = B * Hkv * p.tiles;
-  int64_t keys = (max_ctx * groups + 1023) / 1024;
+  int64_t keys = (max_ctx * groups + 511) / 512;
   keys = (keys + 127) / 128 * 128;
   if (keys < 128) keys = 128;
-  if (keys > 2048 && groups < 512) keys = 2048;
-  if (groups >= 512) keys = (max_ctx + 127) / 128 * 128;
+  if (p.mt < 8 && keys > 512) keys = 512;
+  if (keys > max_ctx) keys = (max_ctx + 127) / 128 * 128;
   p.split_keys = (int)keys;
   p.splits = (int)((max_ctx + keys - 1) / keys);
   return p;
@@ -790,8 +834,13 @@ extern "C" int zk_attn_paged(const void* q, const void* k_cache, const void* v_c
                       : (p.mt == 1 ? attn_paged_stream_kernel<64, 1> : p.mt == 2 ? attn_paged_stream_kernel<64, 2> : one_page ? attn_paged_tile_kernel<64, true> : attn_paged_tile_kernel<64, false>);
   hipLaunchKernelGGL(kern, dim3((unsigned)((groups + 7) / 8 * 8 * p.tiles)), dim3(256), 0, stream, a);
   if (p.splits > 1) {
-    void (*merge)(PagedArgs) = head_dim == 128 ? attn_paged_merge_kernel<128> : attn_paged_merge_kernel<64>;
-    hipLaunchKernelGGL(merge, dim3((unsigned)(T * Hq)), dim3((unsigned)head_dim), 0, stream, a);
+    // few shares: a wave a row; many of few rows: four (two) workgroups a row
+    const bool few = p.splits <= 16, slices = p.splits > 64 && T * Hq < 256;
+    void (*merge)(PagedArgs) =
+        head_dim == 128 ? (few ? attn_paged_merge_few_kernel<128> : slices ? attn_paged_merge_kernel<128, 32> : attn_paged_merge_kernel<128, 128>)
+                        : (few ? attn_paged_merge_few_kernel<64> : slices ? attn_paged_merge_kernel<64, 32> : attn_paged_merge_kernel<64, 64>);
+    const int64_t wgs = few ? (T * Hq + 3) / 4 : T * Hq * (slices ? head_dim / 32 : 1);
+    hipLaunchKernelGGL(merge, dim3((unsigned)wgs), dim3(kMergeThreads), 0, stream, a);
   }
   ZK_CHECK_LAUNCH();
   return ZK_OK;
