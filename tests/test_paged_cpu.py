@@ -82,3 +82,82 @@ def test_wrappers_refuse_host_tensors():
         ops.kv_append_paged(b(2, 512), torch.zeros(4, 32), torch.zeros(4, 32), b(2, 4, 128), b(2, 4, 128), i(2), i(2), 4, 2, 64)
     with pytest.raises(ValueError, match="device"):
         ops.attn_paged(b(2, 256), b(2, 4, 128), b(2, 4, 128), i(2).view(1, 2), i(1), i(2), 2, 8, 4, 2, 64, 0.1)
+
+
+# ---- the host side of the paged cache -------------------------------------------------------------------------------
+def cache_of(**kw):
+    from zero_amd.inference.paged import PagedKVCache
+    a = dict(n_layers=2, max_seqs=3, max_len=20, kv_width=8, device="cpu", page_size=4)
+    a.update(kw)
+    return PagedKVCache(**a)
+
+
+def test_cache_hands_out_pages_and_takes_them_back():
+    c = cache_of(n_pages=6)
+    st = c.step([5, 0, 9])                                    # 2 + 0 + 3 pages
+    assert [len(p) for p in c.pages] == [2, 0, 3] and len({p for ps in c.pages for p in ps}) == 5
+    assert st.cu == [0, 5, 5, 14] and st.max_q == 9 and st.max_ctx == 9 and st.mask is None
+    assert st.positions.tolist() == list(range(5)) + list(range(9)) and st.ctx_lens.tolist() == [5, 0, 9]
+    assert st.slots.tolist() == [c.row(0, r) for r in range(5)] + [c.row(2, r) for r in range(9)]
+    assert len(set(st.slots.tolist())) == 14
+    for b, ps in enumerate(c.pages):
+        assert c.page_table[b].tolist() == ps + [-1] * (5 - len(ps))
+    assert c.lengths == [0, 0, 0]
+    c.advance([5, 0, 9])
+    nxt = c.step([1, 1, 1])                                   # 5 -> 6 and 9 -> 10 fit their pages; sequence 1 takes the last
+    assert nxt.positions.tolist() == [5, 0, 9] and len(c._free) == 0
+    with pytest.raises(RuntimeError, match="out of pages"):
+        c.step([4, 0, 0])                                     # 9 rows: a third page
+    c.advance([1, 1, 1])
+    c.truncate(2, 4)
+    assert c.lengths == [6, 1, 4] and len(c._free) == 2 and c.page_table[2].tolist() == c.pages[2] + [-1] * 4
+    c.release(0)
+    assert c.lengths[0] == 0 and len(c._free) == 4
+    with pytest.raises(ValueError, match="too small"):
+        c.step([21, 0, 0])
+    for bad in ([0, 0, 0], [1, 1]):
+        with pytest.raises(ValueError):
+            c.step(bad)
+    with pytest.raises(ValueError):
+        c.step([2, 0, 0], [[-1], [], []])
+    with pytest.raises(ValueError):
+        cache_of(page_size=0)
+
+
+def test_cache_keeps_a_path_of_a_tree():
+    """Rows of the path move to the front, over pages, for all layers; sources that are destinations of others first read."""
+    c = cache_of(max_seqs=2, page_size=3)
+    c.kv.fill_(0.5)                                           # (fresh memory may hold NaN, which equals nothing)
+    c.step([4, 2]); c.advance([4, 2])
+    trees = [[-1, 0, 0, 1, 2, 3, 4], [-1]]
+    st = c.step([7, 1], trees)
+    assert st.positions.tolist() == [4, 5, 5, 6, 6, 7, 7, 2]
+    rows = c.kv.view(2, 2, -1, 8)
+    for i, s in enumerate(st.slots.tolist()):
+        rows[:, :, s] = float(i + 1)
+    before = rows[:, :, [c.row(0, r) for r in range(4)]].clone()
+    c.keep([[0, 2, 4, 6], [0]])
+    assert c.lengths == [8, 3] and len(c.pages[0]) == 3
+    got = [rows[:, :, c.row(0, 4 + d)].unique().tolist() for d in range(4)]
+    assert got == [[1.0], [3.0], [5.0], [7.0]]
+    assert torch.equal(rows[:, :, [c.row(0, r) for r in range(4)]], before)
+    c.keep([[], [0]])                                          # a finished sequence keeps nothing
+    assert c.lengths == [8, 4]
+
+
+def test_tree_masks_and_paths():
+    from zero_amd.inference.paged import accepted_path, ancestors, depths, draft_tree, tree_mask
+    assert draft_tree(2, 3) == [-1, 0, 0, 1, 2, 3, 4] and draft_tree(3, 0) == [-1]
+    assert depths(draft_tree(2, 3)) == [0, 1, 1, 2, 2, 3, 3]
+    assert ancestors([-1, 0, 0, 1]) == [0b1, 0b11, 0b101, 0b1011]
+    with pytest.raises(ValueError):
+        ancestors([-1, 1])
+    m = tree_mask([[-1, 0], list(range(-1, 129))], "cpu")     # a pair, and a chain of 130: three words
+    assert tuple(m.shape) == (132, 3) and m[1].tolist() == [3, 0, 0]
+    assert m[2 + 129].tolist() == [-1, -1, 3] and m[2 + 63].tolist() == [-1, 0, 0]
+    t = draft_tree(2, 2)                                      # root, a b, a' b'
+    tok = [9, 4, 5, 6, 7]
+    assert accepted_path(t, tok, [5, 0, 7, 0, 1]) == [0, 2, 4]
+    assert accepted_path(t, tok, [4, 7, 7, 0, 1]) == [0, 1]
+    assert accepted_path(t, tok, [3, 6, 7, 0, 1]) == [0]
+    assert accepted_path([-1, 0, 0], [1, 2, 2], [2, 0, 0]) == [0, 1]

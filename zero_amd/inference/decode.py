@@ -1,5 +1,6 @@
 """Inference through the decoder with a KV cache: prefill (the training path's causal attention
-kernel) + greedy decoding (single-query attention over the cache), optionally tensor parallel.
+kernel) + decoding of one token a step (single-query attention over the cache), greedy or sampled, optionally tensor
+parallel.  Prompts of different lengths and drafted decoding go through inference.paged.
 
 Mirrors what the reference gets from ``transformers`` in ref:inference/vlm_infer.py:259-270:
 ``decoder.generate(inputs_embeds=…, attention_mask=ones, do_sample=False, max_new_tokens=…,
@@ -43,16 +44,13 @@ def _gate_up_interleaved(gw, uw):
     return cache["wi"]
 
 
-@torch.no_grad()
-def layer_infer(layer, x2: torch.Tensor, B: int, S: int, pos0: int, cos_t, sin_t, cache: KVCache, li: int,
-                tp: TPContext) -> torch.Tensor:
-    """One decoder layer (tf:llama:295-324) on rows x2 [B*S, d]; positions pos0 .. pos0+S-1."""
-    a, m = layer.self_attn, layer.mlp
+def qkv_infer(layer, x2: torch.Tensor) -> torch.Tensor:
+    """Packed q|k|v rows [M, (nh + 2 nkv) * hd] (local heads) of the layer's normalised input, before RoPE."""
+    a = layer.self_attn
     _, _, hd, eps = layer.cfg_dims
     nh, nkv = a.q_proj.weight.shape[0] // hd, a.k_proj.weight.shape[0] // hd      # local (sharded) head counts
-    M, d = x2.shape
     h1, _ = ops.rmsnorm_fwd(x2, layer.input_layernorm.weight, eps, save_stats=False)
-    qkv = torch.empty((M, (nh + 2 * nkv) * hd), dtype=BF16, device=x2.device)
+    qkv = torch.empty((x2.shape[0], (nh + 2 * nkv) * hd), dtype=BF16, device=x2.device)
     wqkv = ZF.packed_rows(a.q_proj.weight, a.k_proj.weight, a.v_proj.weight)
     if wqkv is not None:
         ops.gemm(h1, wqkv.detach(), out=qkv)
@@ -60,19 +58,12 @@ def layer_infer(layer, x2: torch.Tensor, B: int, S: int, pos0: int, cos_t, sin_t
         ops.gemm(h1, a.q_proj.weight.detach(), out=qkv[:, :nh * hd])
         ops.gemm(h1, a.k_proj.weight.detach(), out=qkv[:, nh * hd:(nh + nkv) * hd])
         ops.gemm(h1, a.v_proj.weight.detach(), out=qkv[:, (nh + nkv) * hd:])
-    # row r of qkv is position pos0 + r % S: hand the kernel the table rows from pos0 on
-    ops.rope_(qkv, cos_t[pos0:pos0 + S], sin_t[pos0:pos0 + S], S, nh + nkv, hd)
-    q, k, v = qkv[:, :nh * hd], qkv[:, nh * hd:(nh + nkv) * hd], qkv[:, (nh + nkv) * hd:]
-    cache.k[li][:, pos0:pos0 + S].copy_(k.view(B, S, nkv * hd))
-    cache.v[li][:, pos0:pos0 + S].copy_(v.view(B, S, nkv * hd))
-    if S > 1:
-        if pos0 != 0:
-            raise NotImplementedError("chunked prefill (S > 1 on a non-empty cache)")
-        ao, _ = ops.attn_fwd(q, k, v, B, S, nh, nkv, hd, hd ** -0.5, True, need_lse=False)
-    else:
-        ao = ops.attn_decode(q, cache.k[li], cache.v[li], cache.lens, pos0 + 1, nh, nkv, hd, hd ** -0.5)
-    # row-parallel projections: every rank holds a slice of the contraction; ONE rank adds the residual
-    xa = tp.reduce(ops.gemm(ao, a.o_proj.weight.detach(), residual=x2 if tp.lead else None))
+    return qkv
+
+
+def mlp_infer(layer, xa: torch.Tensor, tp: TPContext) -> torch.Tensor:
+    """The layer's MLP half with its residual."""
+    m, eps, M = layer.mlp, layer.cfg_dims[3], xa.shape[0]
     h2, _ = ops.rmsnorm_fwd(xa, layer.post_attention_layernorm.weight, eps, save_stats=False)
     gw, uw = m.gate_proj.weight, m.up_proj.weight
     wgu = ZF.packed_rows(gw, uw)
@@ -83,11 +74,35 @@ def layer_infer(layer, x2: torch.Tensor, B: int, S: int, pos0: int, cos_t, sin_t
         _, hm = ops.gemm_swiglu(h2, _gate_up_interleaved(gw, uw), keep_gu=False)   # prefill: h only
     else:
         F = gw.shape[0]
-        gu = torch.empty((M, 2 * F), dtype=BF16, device=x2.device)
+        gu = torch.empty((M, 2 * F), dtype=BF16, device=xa.device)
         ops.gemm(h2, gw.detach(), out=gu[:, :F])
         ops.gemm(h2, uw.detach(), out=gu[:, F:])
         hm = ops.swiglu_fwd(gu, F)
     return tp.reduce(ops.gemm(hm, m.down_proj.weight.detach(), residual=xa if tp.lead else None))
+
+
+@torch.no_grad()
+def layer_infer(layer, x2: torch.Tensor, B: int, S: int, pos0: int, cos_t, sin_t, cache: KVCache, li: int,
+                tp: TPContext) -> torch.Tensor:
+    """One decoder layer (tf:llama:295-324) on rows x2 [B*S, d]; positions pos0 .. pos0+S-1."""
+    a = layer.self_attn
+    _, _, hd, _ = layer.cfg_dims
+    nh, nkv = a.q_proj.weight.shape[0] // hd, a.k_proj.weight.shape[0] // hd      # local (sharded) head counts
+    qkv = qkv_infer(layer, x2)
+    # row r of qkv is position pos0 + r % S: hand the kernel the table rows from pos0 on
+    ops.rope_(qkv, cos_t[pos0:pos0 + S], sin_t[pos0:pos0 + S], S, nh + nkv, hd)
+    q, k, v = qkv[:, :nh * hd], qkv[:, nh * hd:(nh + nkv) * hd], qkv[:, (nh + nkv) * hd:]
+    cache.k[li][:, pos0:pos0 + S].copy_(k.view(B, S, nkv * hd))
+    cache.v[li][:, pos0:pos0 + S].copy_(v.view(B, S, nkv * hd))
+    if S > 1:
+        if pos0 != 0:
+            raise NotImplementedError("chunked prefill (S > 1 on a non-empty cache): inference.paged.forward_paged")
+        ao, _ = ops.attn_fwd(q, k, v, B, S, nh, nkv, hd, hd ** -0.5, True, need_lse=False)
+    else:
+        ao = ops.attn_decode(q, cache.k[li], cache.v[li], cache.lens, pos0 + 1, nh, nkv, hd, hd ** -0.5)
+    # row-parallel projections: every rank holds a slice of the contraction; ONE rank adds the residual
+    xa = tp.reduce(ops.gemm(ao, a.o_proj.weight.detach(), residual=x2 if tp.lead else None))
+    return mlp_infer(layer, xa, tp)
 
 
 class DecodePlan:
@@ -190,31 +205,70 @@ def forward_cached(decoder, x: torch.Tensor, cache: KVCache, tp: Optional[TPCont
     return logits.view(B, 1 if last_only else S, -1)
 
 
-@torch.no_grad()
-def generate(decoder, inputs_embeds: torch.Tensor, attention_mask=None, do_sample: bool = False,
-             max_new_tokens: int = 20, use_cache: bool = True, eos_token_id=None, pad_token_id=None,
-             tp: Optional[TPContext] = None) -> torch.Tensor:
-    """Greedy decoding from prompt embeddings; returns the new token ids [B, <= max_new_tokens] (int64)."""
-    if do_sample:
-        raise NotImplementedError("sampling: the reference decodes greedily (ref:vlm_infer.py:267)")
-    if attention_mask is not None and not bool((attention_mask != 0).all()):
-        raise NotImplementedError("attention masks with holes: the reference passes all ones (ref:vlm_infer.py:260-263)")
+def eos_ids(decoder, eos_token_id=None, pad_token_id=None):
+    """(set of EOS ids, pad id or None) from the arguments or the decoder's generation_config."""
     gc = getattr(decoder, "generation_config", None)
     eos = eos_token_id if eos_token_id is not None else getattr(gc, "eos_token_id", None)
     pad = pad_token_id if pad_token_id is not None else getattr(gc, "pad_token_id", None)
     eos_set = set() if eos is None else set(eos if isinstance(eos, (list, tuple)) else [eos])
     if pad is None and eos_set:
         pad = sorted(eos_set)[0]
+    return eos_set, pad
+
+
+def draw_tokens(logits: torch.Tensor, u: Optional[torch.Tensor], sampling: Optional[dict]) -> torch.Tensor:
+    """Next tokens [rows] from logits [rows, V]: the largest (tf: argmax of the fp32 scores), or ops.sample's."""
+    if sampling is None:
+        return logits.float().argmax(-1)
+    return ops.sample(logits, u, **sampling)[0]
+
+
+def check_drawn(tokens: List[int]) -> List[int]:
+    if min(tokens, default=0) < 0:
+        raise FloatingPointError("sampling: a row of logits without a token that can be drawn (NaN, or nothing but -inf)")
+    return tokens
+
+
+@torch.no_grad()
+def generate(decoder, inputs_embeds: torch.Tensor, attention_mask=None, do_sample: bool = False,
+             max_new_tokens: int = 20, use_cache: bool = True, eos_token_id=None, pad_token_id=None,
+             tp: Optional[TPContext] = None, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+             min_p: float = 0.0, generator: Optional[torch.Generator] = None, assistant=None, draft_width: int = 2,
+             draft_depth: int = 4) -> torch.Tensor:
+    """Decoding from prompt embeddings [B, S, d]; returns the new token ids [B, <= max_new_tokens] (int64).
+
+    Greedy, or with ``do_sample`` by ops.sample's temperature / top_k / top_p / min_p from uniform numbers of ``generator``
+    (a device generator; under tensor parallelism every rank passes one of equal seed).  ``attention_mask`` [B, S]: positions
+    with 0 are left out, so prompts of different lengths decode as they would alone.  ``assistant``: a decoder of the same
+    vocabulary and width that drafts ``draft_width`` chains of ``draft_depth`` tokens a step; greedy tokens stay those of
+    decoding without it and sampled ones follow the same distributions, up to the rounding of products with other row
+    counts."""
+    sampling = dict(temperature=float(temperature), top_k=int(top_k), top_p=float(top_p), min_p=float(min_p)) if do_sample else None
+    keep = None if attention_mask is None else attention_mask != 0
+    ragged = keep is not None and not bool(keep.all())
+    if ragged or assistant is not None:
+        from .paged import generate_paged
+        if keep is not None and keep.shape != inputs_embeds.shape[:2]:
+            raise ValueError(f"attention_mask {tuple(keep.shape)} for prompts {tuple(inputs_embeds.shape[:2])}")
+        prompts = [x if keep is None else x[k.to(x.device)] for x, k in
+                   zip(inputs_embeds, keep if keep is not None else [None] * inputs_embeds.shape[0])]
+        return generate_paged(decoder, prompts, max_new_tokens, eos_token_id, pad_token_id, sampling, generator, assistant,
+                              draft_width, draft_depth, tp=tp)
+    eos_set, pad = eos_ids(decoder, eos_token_id, pad_token_id)
     B, S, d = inputs_embeds.shape
+    u = torch.rand((max_new_tokens, B), generator=generator, device=inputs_embeds.device) if sampling is not None else None
     a0 = decoder.model.layers[0].self_attn
     cache = KVCache(len(decoder.model.layers), B, S + max_new_tokens, a0.k_proj.weight.shape[0], inputs_embeds.device)
     wte = decoder.model.get_input_embeddings()
     out: List[torch.Tensor] = []
     done = torch.zeros(B, dtype=torch.bool, device=inputs_embeds.device)
+    undrawn = torch.zeros(B, dtype=torch.bool, device=inputs_embeds.device)
     x = inputs_embeds
-    for _ in range(max_new_tokens):
+    for i in range(max_new_tokens):
         logits = forward_cached(decoder, x, cache, tp)                    # [B, 1, V]
-        nxt = logits[:, 0].float().argmax(-1)                             # greedy (tf: argmax of the fp32 scores)
+        nxt = draw_tokens(logits[:, 0], None if u is None else u[i], sampling)
+        if sampling is not None:
+            undrawn |= (nxt < 0) & ~done
         if eos_set:
             nxt = torch.where(done, torch.full_like(nxt, pad), nxt)
         out.append(nxt)
@@ -225,5 +279,7 @@ def generate(decoder, inputs_embeds: torch.Tensor, attention_mask=None, do_sampl
             done |= hit
             if bool(done.all()):
                 break
-        x = wte(nxt.view(B, 1))
+        x = wte(nxt.view(B, 1))                                           # (a token of -1 reads a row of zeros)
+    if sampling is not None and bool(undrawn.any()):
+        check_drawn([-1])
     return torch.stack(out, dim=1)

@@ -36,9 +36,10 @@ def graft_inputs(model, imgs: List[torch.Tensor], input_ids: Sequence[Sequence[i
 
 @torch.no_grad()
 def graft_generate(model, imgs: List[torch.Tensor], input_ids: Sequence[Sequence[int]], img_id: int,
-                   max_new_tokens: int = 1024, tp: Optional[TPContext] = None, **gen_kwargs) -> torch.Tensor:
-    """New token ids [B, <= max_new_tokens] (greedy, KV cache), ref:vlm_infer.py:259-270."""
+                   max_new_tokens: int = 1024, tp: Optional[TPContext] = None, do_sample: bool = False,
+                   **gen_kwargs) -> torch.Tensor:
+    """New token ids [B, <= max_new_tokens] (KV cache; greedy unless ``do_sample``), ref:vlm_infer.py:259-270."""
     x = graft_inputs(model, imgs, input_ids, img_id)
     mask = torch.ones(x.shape[:2], device=x.device)                      # vlm_infer.py:260-263
-    return generate(model.decoder, x, attention_mask=mask, do_sample=False, max_new_tokens=max_new_tokens,
+    return generate(model.decoder, x, attention_mask=mask, do_sample=do_sample, max_new_tokens=max_new_tokens,
                     use_cache=True, tp=tp, **gen_kwargs)
