@@ -94,8 +94,11 @@ struct PagedArgs {
   bf16_t* out;
   const int *table, *ctx, *cu;
   const unsigned long long* mask;
-  float *part_o, *part_ml;      // [T * Hq][splits][HD] un-normalised outputs, [..][2] maximum and sum; null: one split
-  int T, B, Hq, Hkv, page_size, n_pages, table_cols, ld_table, mask_words;
+  // shares' un-normalised outputs and (maximum, sum): [T * Hq][splits][HD], [..][2] (stream kernel) or
+  // [workgroup][128 rows][HD], [..][2] with the layout in `shares` (tile kernel); null: no sequence is shared out
+  float *part_o, *part_ml;
+  int* shares;
+  int T, B, max_q, Hq, Hkv, page_size, n_pages, table_cols, ld_table, mask_words;
   int tiles, splits, split_keys, groups;
   unsigned page_mul, page_shift;   // key / page_size = key * page_mul >> page_shift for every key < 2^31
   long long ldq, ldo;
@@ -108,12 +111,14 @@ constexpr int kMaxRows = 1 << 30;
 struct Seq {
   int q0, n, len;               // first row of q, new tokens, cached rows
   int first;                    // cached rows before the new tokens (as the lengths say: negative if they do not fit)
+  int rows;                     // of a kv head: computed tokens times the heads that share it
   __device__ __forceinline__ Seq(const PagedArgs& a, int b) {
     q0 = min(max(a.cu[b], 0), a.T);
     n = min(max(a.cu[b + 1], q0), a.T) - q0;
     const int c = min(max(a.ctx[b], 0), kMaxRows);  // and T < kMaxRows: differences of the two fit 32 bits
     len = (int)min((long long)c, (long long)a.table_cols * a.page_size);
     first = c - n;
+    rows = min(n, a.max_q) * (a.Hq / a.Hkv);
   }
 };
 
@@ -169,6 +174,89 @@ struct Work {
   }
 };
 
+// Shares of the tile kernel's work, from the lengths themselves (the host knows bounds only; shares cut by the largest
+// length left half of the CUs idle on a ragged batch).  A share is `q` 64-key tiles of one (sequence, kv head, 128-row
+// tile); q is the cut of the longest sequence into 1 .. 64 that minimises rounds * (q + 4), 4 tiles being what a share costs
+// beside its own (prologue, stores, merge), with the workgroups that the GPU holds at once as a round.  Each wave works
+// it out for itself, lane i trying the cut into i + 1.  Workgroup ids run over sequences, row tiles, shares, kv heads:
+// with 8 kv heads the row tiles of a share are on one XCD (ids equal modulo 8) and its L2 serves all but the first.
+template <int HD>
+constexpr int kTileSlots = HD == 64 ? 768 : 512;    // three / two workgroups a CU
+struct Shares {
+  int q, b = -1, tile = 0, unit = 0, units = 0;     // unit = share * Hkv + kv head, of `units`; b < 0: no work
+  __device__ __forceinline__ static void of(const PagedArgs& a, int b, int& tiles, int& len) {
+    tiles = len = 0;
+    if (b >= a.B) return;
+    const Seq s(a, b);
+    tiles = (s.rows + 127) >> 7;
+    len = max((s.len + 63) >> 6, 1);
+  }
+  __device__ __forceinline__ Shares(const PagedArgs& a, int slots, int id) {
+    const int lane = threadIdx.x & 63;
+    int tiles, len, all = 0, longest = 1;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+      of(a, b0 + lane, tiles, len);
+      all += tiles;
+      longest = max(longest, tiles ? len : 1);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) { all += __shfl_xor(all, o, 64); longest = max(longest, __shfl_xor(longest, o, 64)); }
+    all *= a.Hkv;
+    q = longest;
+    if (a.part_o && longest > 4 && all < 2 * slots) {
+      const int mine = (longest + lane) / (lane + 1);
+      const float inv = 1.0f / (float)mine;
+      int n = 0;
+      for (int b0 = 0; b0 < a.B; b0 += 64) {
+        if (a.B > 64) of(a, b0 + lane, tiles, len);
+        for (int j = 0; j < min(64, a.B - b0); ++j)
+          n += __builtin_amdgcn_readlane(tiles, j) * (int)(((float)(__builtin_amdgcn_readlane(len, j) + mine) - 0.5f) * inv);
+      }
+      n *= a.Hkv;
+      int cost = (n + slots - 1) / slots * (mine + 4);
+      if (n > 2 * slots && lane) cost = 0x1FFFFFF;
+      int best = (min(cost, 0x1FFFFFF) << 6) | lane;
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) best = min(best, __shfl_xor(best, o, 64));
+      q = (longest + (best & 63)) / ((best & 63) + 1);
+    }
+    for (;;) {
+      b = -1;
+      int before = 0;
+      for (int b0 = 0; b0 < a.B; b0 += 64) {
+        if (a.B > 64) of(a, b0 + lane, tiles, len);
+        const int u = a.Hkv * ((len + q - 1) / q), n = tiles * u;
+        int upto = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const int y = __shfl_up(upto, o, 64);
+          if (lane >= o) upto += y;
+        }
+        const int start = before + upto - n;
+        if (id == 0 && threadIdx.x < 64 && a.part_o && b0 + lane < a.B) a.shares[1 + b0 + lane] = start;
+        const unsigned long long hit = __ballot(id >= start && id < start + n);
+        if (hit) {
+          const int at = __ffsll(hit) - 1;
+          b = b0 + at;
+          units = __builtin_amdgcn_readlane(u, at);
+          unit = id - __builtin_amdgcn_readlane(start, at);
+          tile = unit / units;
+          unit -= tile * units;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+      }
+      if (q == longest || before <= 2 * slots) break;
+      q = longest;                                  // (the choice above counts in fp32)
+    }
+    if (id == 0 && threadIdx.x == 0 && a.part_o) a.shares[0] = q == longest ? 0 : q;
+    q = __builtin_amdgcn_readfirstlane(q);          // (all of these are the same in the workgroup)
+    b = __builtin_amdgcn_readfirstlane(b);
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    unit = __builtin_amdgcn_readfirstlane(unit);
+    units = __builtin_amdgcn_readfirstlane(units);
+  }
+};
+
 __device__ __forceinline__ bool not_finite(unsigned w) {
   return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
 }
@@ -201,7 +289,7 @@ __global__ __launch_bounds__(256, MT == 1 && HD == 64 ? 4 : 2) void attn_paged_s
   if (!w.any) return;
   const int kvh = w.kvh, tile = w.tile, split = w.split, b = w.b;
   const Seq s(a, b);
-  const int G = a.Hq / a.Hkv, rows = s.n * G, r0 = tile * 16 * MT, kvw = a.Hkv * HD;
+  const int G = a.Hq / a.Hkv, rows = s.rows, r0 = tile * 16 * MT, kvw = a.Hkv * HD;
   const int ks = split * a.split_keys;
   if (r0 >= rows || (split > 0 && ks >= s.len)) return;
   const int ke = split == a.splits - 1 ? s.len : min(s.len, ks + a.split_keys);
@@ -447,22 +535,20 @@ __device__ __forceinline__ void lds_dma_at(const void* dst, const void* base, un
 // ONE_PAGE: page_size is a multiple of 64, so a tile lies in one page: its address is uniform and a lane's offset into it
 // constant, where pages of any size cost a look-up, four exchanges and 64-bit multiplies a lane and tile.
 template <int HD, bool ONE_PAGE>
-__global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedArgs a) {
+__global__ __launch_bounds__(256, kTileSlots<HD> / 256) void attn_paged_tile_kernel(PagedArgs a) {
   using C = Cfg<HD>;
   constexpr int KV = 64, RB = HD * 2, TB = KV * RB, STAGE = 2 * TB, CPR = HD / 8, NQ = KV * CPR / 256;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * STAGE];
   __shared__ unsigned bad[2];
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Work w(a);
-  if (!w.any) return;
-  const int kvh = w.kvh, b = w.b, split = w.split;
+  const Shares w(a, kTileSlots<HD>, (int)blockIdx.x);
+  if (w.b < 0) return;
+  const int b = w.b, split = __builtin_amdgcn_readfirstlane(w.unit / a.Hkv), kvh = w.unit - split * a.Hkv;
   const Seq s(a, b);
-  const int G = a.Hq / a.Hkv, rows = s.n * G, kvw = a.Hkv * HD, t0 = w.tile * 128;
-  const int ks = split * a.split_keys;
-  if (t0 >= rows || (split > 0 && ks >= s.len)) return;
-  const int ke = split == a.splits - 1 ? s.len : min(s.len, ks + a.split_keys);
-  const bool alone = ks == 0 && ke == s.len;
+  const int G = a.Hq / a.Hkv, rows = s.rows, kvw = a.Hkv * HD, t0 = w.tile * 128;
+  const int ks = split * w.q * KV, ke = min(s.len, ks + w.q * KV);
+  const bool alone = w.units == a.Hkv;
   const float sc = a.scale * kLog2e;
   const int r0 = t0 + wave * 32, r = r0 + (lane & 31), rc = min(r, rows - 1), tok = rc / G;
   // keys that the workgroup / this wave needs at all, and those that every row of the workgroup sees
@@ -643,7 +729,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedArgs a) {
         *reinterpret_cast<u32x2*>(op + d * 32 + 8 * r4 + 4 * h) = y;
       }
   } else {
-    const size_t part = ((size_t)tq * a.Hq + head) * a.splits + split;
+    const size_t part = (size_t)blockIdx.x * 128 + (r - t0);
 #pragma unroll
     for (int d = 0; d < C::DB; ++d)
 #pragma unroll
@@ -666,7 +752,7 @@ __global__ __launch_bounds__(kMergeThreads) void attn_paged_merge_kernel(PagedAr
   __shared__ float red[4], sum[4];
   const int id = blockIdx.x / NSL, t = id / a.Hq, h = id % a.Hq, col0 = blockIdx.x % NSL * COLS, tid = threadIdx.x;
   const Seq s(a, seq_of(a, t));
-  if (t < s.q0 || t >= s.q0 + s.n) return;
+  if (t < s.q0 || t >= s.q0 + min(s.n, a.max_q)) return;
   const int parts = min(a.splits, (s.len + a.split_keys - 1) / a.split_keys);
   if (parts <= 1) return;                           // written by its only share
   const float* ml = a.part_ml + (size_t)id * a.splits * 2;
@@ -717,7 +803,7 @@ __global__ __launch_bounds__(256) void attn_paged_merge_few_kernel(PagedArgs a) 
   if (id >= a.T * a.Hq) return;
   const int t = id / a.Hq, h = id % a.Hq;
   const Seq s(a, seq_of(a, t));
-  if (t < s.q0 || t >= s.q0 + s.n) return;
+  if (t < s.q0 || t >= s.q0 + min(s.n, a.max_q)) return;
   const int parts = min(a.splits, (s.len + a.split_keys - 1) / a.split_keys);
   if (parts <= 1) return;
   const float* ml = a.part_ml + (size_t)id * a.splits * 2;
@@ -730,7 +816,6 @@ __global__ __launch_bounds__(256) void attn_paged_merge_few_kernel(PagedArgs a) 
   float y[CPL];
 #pragma unroll
   for (int c = 0; c < CPL; ++c) y[c] = 0.f;
-#pragma unroll 4
   for (int i = 0; i < parts; ++i) {
     const float w = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(f), i));
 #pragma unroll
@@ -741,27 +826,73 @@ __global__ __launch_bounds__(256) void attn_paged_merge_few_kernel(PagedArgs a) 
   else *op = f2bf(y[0] * inv);
 }
 
+// the same for the tile kernel's shares: a wave a row in turn
+template <int HD>
+__global__ __launch_bounds__(256) void attn_paged_merge_tiles_kernel(PagedArgs a) {
+  constexpr int CPL = HD / 64;
+  const int q = a.shares[0];
+  if (!q) return;                                   // no sequence was shared out
+  const int lane = threadIdx.x & 63, G = a.Hq / a.Hkv;
+  for (int id = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6))); id < a.T * a.Hq; id += (int)gridDim.x * 4) {
+    const int t = id / a.Hq, h = id % a.Hq, b = seq_of(a, t);
+    const Seq s(a, b);
+    const int i = t - s.q0, parts = (((s.len + 63) >> 6) + q - 1) / q;
+    if (i < 0 || i >= min(s.n, a.max_q) || parts <= 1) continue;
+    const int r = i * G + h % G;
+    const size_t p0 = (size_t)(a.shares[1 + b] + (r >> 7) * parts * a.Hkv + h / G) * 128 + (r & 127), step = (size_t)a.Hkv * 128;
+    const float* ml = a.part_ml + 2 * (p0 + lane * step);
+    const float m = lane < parts ? ml[0] : -INFINITY, l = lane < parts ? ml[1] : 0.f;
+    const float M = wave_max(m);
+    const float f = M == -INFINITY ? 0.f : fast_exp2(m - M);
+    const float L = wave_sum(l * f);
+    const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
+    float y[CPL];
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) y[c] = 0.f;
+    for (int j = 0; j < parts; ++j) {
+      const float w = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(f), j));
+      const float* po = a.part_o + (p0 + j * step) * HD + lane * CPL;
+#pragma unroll
+      for (int c = 0; c < CPL; ++c) y[c] += po[c] * w;
+    }
+    bf16_t* op = a.out + (size_t)t * a.ldo + (size_t)h * HD + lane * CPL;
+    if (CPL == 2) *reinterpret_cast<unsigned*>(op) = pack2bf(y[0] * inv, y[CPL - 1] * inv);
+    else *op = f2bf(y[0] * inv);
+  }
+}
+
 // shape of a launch: host arithmetic on the sizes alone
 struct Plan {
   int mt, tiles, splits, split_keys;                // mt: 16-row groups of the stream kernel's tile, 8 = the tile kernel
+  int64_t grid, header, parts, ws;                  // workgroups; floats of the header, parts, floats altogether
 };
-inline Plan plan_of(int64_t B, int64_t max_q, int64_t max_ctx, int64_t Hq, int64_t Hkv) {
-  Plan p;
+inline Plan plan_of(int64_t B, int64_t T, int64_t max_q, int64_t max_ctx, int64_t Hq, int64_t Hkv, int64_t hd) {
+  Plan p{};
   const int64_t rows = max_q * (Hq / Hkv);
   p.mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 8;
   p.tiles = (int)((rows + 16 * p.mt - 1) / (16 * p.mt));
-  // shares of the keys: as many as fill the 512 workgroups that the CUs hold at two each, none under 128 keys (a piece for
-  // each wave).  The stream kernel's shares end at 512 keys: the lengths of a batch differ, and small shares even that out
-  // (48 sequences of 700 to 8192: 150 us with 1024 keys, 140 with 512).  The tile kernel's do not: a share costs it a
-  // prologue of several tiles and 130 floats a row through memory.
   const int64_t groups = B * Hkv * p.tiles;
-  int64_t keys = (max_ctx * groups + 511) / 512;
-  keys = (keys + 127) / 128 * 128;
-  if (keys < 128) keys = 128;
-  if (p.mt < 8 && keys > 512) keys = 512;
-  if (keys > max_ctx) keys = (max_ctx + 127) / 128 * 128;
-  p.split_keys = (int)keys;
-  p.splits = (int)((max_ctx + keys - 1) / keys);
+  if (p.mt == 8) {
+    // shares are cut on the device; no sequence of up to four 64-key tiles is, nor any where there is work for two rounds
+    const int64_t slots = hd == 64 ? kTileSlots<64> : kTileSlots<128>;
+    const bool shared = max_ctx > 256 && T * Hq < 128 * 2 * slots;
+    p.splits = shared ? 2 : 1;
+    p.grid = shared && groups < 2 * slots ? 2 * slots : groups;
+    p.header = shared ? (B + 64) / 64 * 64 : 0;
+    p.parts = shared ? 2 * slots * 128 : 0;
+  } else {
+    // shares of the keys: as many as fill the 512 workgroups that the CUs hold at two each, none under 128 keys (a piece
+    // for each wave) and none over 512: the lengths of a batch differ, and small shares even that out (48 sequences of
+    // 700 to 8192: 150 us with 1024 keys, 140 with 512)
+    int64_t keys = (max_ctx * groups + 511) / 512;
+    keys = (keys + 127) / 128 * 128;
+    keys = keys < 128 ? 128 : keys > 512 ? 512 : keys;
+    p.split_keys = (int)keys;
+    p.splits = (int)((max_ctx + keys - 1) / keys);
+    p.grid = (B * Hkv * p.splits + 7) / 8 * 8 * p.tiles;
+    p.parts = p.splits > 1 ? T * Hq * p.splits : 0;
+  }
+  p.ws = p.header + p.parts * (hd + 2);
   return p;
 }
 
@@ -792,10 +923,9 @@ extern "C" int zk_kv_append_paged(const void* qkv, const float* cos_t, const flo
 extern "C" int zk_attn_paged_ws(int64_t B, int64_t T, int64_t max_q, int64_t max_ctx, int64_t Hq, int64_t Hkv,
                                 int64_t head_dim, int64_t* ws_floats) {
   if (!ws_floats || B <= 0 || T < 0 || max_q <= 0 || max_ctx <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv) return ZK_EINVAL;
-  if ((head_dim != 64 && head_dim != 128) || T > 0x7FFFFFFF || max_q > 0x7FFFFFFF || max_ctx > 0x7FFFFF00) return ZK_EINVAL;
+  if ((head_dim != 64 && head_dim != 128) || T >= kMaxRows || max_q > 0x7FFFFFFF || max_ctx > 0x7FFFFF00) return ZK_EINVAL;
   if (max_q * (Hq / Hkv) > 0x7FFFFFFF || B > 0x7FFFFFFE || T * Hq > 0x7FFFFFFF) return ZK_EINVAL;
-  const Plan p = plan_of(B, max_q, max_ctx, Hq, Hkv);
-  *ws_floats = p.splits > 1 ? T * Hq * p.splits * (head_dim + 2) : 0;
+  *ws_floats = plan_of(B, T, max_q, max_ctx, Hq, Hkv, head_dim).ws;
   return ZK_OK;
 }
 
@@ -809,7 +939,7 @@ extern "C" int zk_attn_paged(const void* q, const void* k_cache, const void* v_c
   const int rc = zk_attn_paged_ws(B, T, max_q, max_ctx, Hq, Hkv, head_dim, &need);
   if (rc != ZK_OK) return rc;
   if (page_size <= 0 || n_pages <= 0 || table_cols <= 0 || ld_table < table_cols) return ZK_EINVAL;
-  if (T >= kMaxRows || B > 0x7FFFFFFE || page_size > 0x7FFFFFFF || n_pages > 0x7FFFFFFF || ld_table > 0x7FFFFFFF) return ZK_EINVAL;
+  if (page_size > 0x7FFFFFFF || n_pages > 0x7FFFFFFF || ld_table > 0x7FFFFFFF) return ZK_EINVAL;
   if (n_pages * page_size > 0x7FFFFFFF || T * Hq > 0x7FFFFFFF || Hkv * head_dim > (1 << 24)) return ZK_EINVAL;
   if ((ldq & 7) || (ldo & 7) || ldq < Hq * head_dim || ldo < Hq * head_dim) return ZK_EINVAL;
   if (!q || !k_cache || !v_cache || !out || !page_table || !ctx_lens || !cu_q) return ZK_EINVAL;
@@ -817,23 +947,27 @@ extern "C" int zk_attn_paged(const void* q, const void* k_cache, const void* v_c
   if (odd16(q) || odd16(k_cache) || odd16(v_cache) || odd16(out) || (need > 0 && (!ws || odd16(ws) || ws_floats < need)))
     return ZK_EINVAL;
   if (T == 0) return ZK_OK;
-  const Plan p = plan_of(B, max_q, max_ctx, Hq, Hkv);
-  const int64_t groups = B * Hkv * p.splits;         // each of p.tiles workgroups
-  if ((groups + 7) * p.tiles > 0x7FFFFFF0) return ZK_EINVAL;
+  const Plan p = plan_of(B, T, max_q, max_ctx, Hq, Hkv, head_dim);
+  if (p.grid > 0x7FFFFFF0) return ZK_EINVAL;
   int lg = 0;                                       // page_mul: the 31-bit reciprocal, rounded up (exact below 2^31)
   while ((int64_t)1 << lg < page_size) ++lg;
   const unsigned mul = (unsigned)((((unsigned long long)1 << (31 + lg)) / (unsigned long long)page_size) + 1);
-  float* part_o = p.splits > 1 ? ws : nullptr;
+  float* part_o = p.splits > 1 ? ws + p.header : nullptr;
   PagedArgs a{(const bf16_t*)q, (const bf16_t*)k_cache, (const bf16_t*)v_cache, (bf16_t*)out, page_table, ctx_lens, cu_q,
-              (const unsigned long long*)tree_mask, part_o, part_o ? ws + T * Hq * p.splits * head_dim : nullptr, (int)T,
-              (int)B, (int)Hq, (int)Hkv, (int)page_size, (int)n_pages, (int)table_cols, (int)ld_table, (int)mask_words,
-              p.tiles, p.splits, p.split_keys, (int)groups, mul, (unsigned)(31 + lg), (long long)ldq, (long long)ldo, scale};
+              (const unsigned long long*)tree_mask, part_o, part_o ? part_o + p.parts * head_dim : nullptr, (int*)ws, (int)T,
+              (int)B, (int)max_q, (int)Hq, (int)Hkv, (int)page_size, (int)n_pages, (int)table_cols, (int)ld_table,
+              (int)mask_words, p.tiles, p.splits, p.split_keys, (int)(B * Hkv * p.splits), mul, (unsigned)(31 + lg),
+              (long long)ldq, (long long)ldo, scale};
   const bool one_page = page_size % 64 == 0;
   void (*kern)(PagedArgs) =
       head_dim == 128 ? (p.mt == 1 ? attn_paged_stream_kernel<128, 1> : p.mt == 2 ? attn_paged_stream_kernel<128, 2> : one_page ? attn_paged_tile_kernel<128, true> : attn_paged_tile_kernel<128, false>)
                       : (p.mt == 1 ? attn_paged_stream_kernel<64, 1> : p.mt == 2 ? attn_paged_stream_kernel<64, 2> : one_page ? attn_paged_tile_kernel<64, true> : attn_paged_tile_kernel<64, false>);
-  hipLaunchKernelGGL(kern, dim3((unsigned)((groups + 7) / 8 * 8 * p.tiles)), dim3(256), 0, stream, a);
-  if (p.splits > 1) {
+  hipLaunchKernelGGL(kern, dim3((unsigned)p.grid), dim3(256), 0, stream, a);
+  if (p.splits > 1 && p.mt == 8) {
+    const int64_t wgs = (T * Hq + 3) / 4;
+    void (*merge)(PagedArgs) = head_dim == 128 ? attn_paged_merge_tiles_kernel<128> : attn_paged_merge_tiles_kernel<64>;
+    hipLaunchKernelGGL(merge, dim3((unsigned)(wgs < 2048 ? wgs : 2048)), dim3(256), 0, stream, a);
+  } else if (p.splits > 1) {
     // few shares: a wave a row; many of few rows: four (two) workgroups a row
     const bool few = p.splits <= 16, slices = p.splits > 64 && T * Hq < 256;
     void (*merge)(PagedArgs) =
