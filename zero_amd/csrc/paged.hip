@@ -794,6 +794,23 @@ __global__ __launch_bounds__(kMergeThreads) void attn_paged_merge_kernel(PagedAr
   a.out[(size_t)t * a.ldo + (size_t)h * HD + col0 + tid] = f2bf(v * inv);
 }
 
+// y += sum_j f[lane j] * x[j * step ..] over up to 64 shares, eight loads in flight; lanes past the last share hold f = 0
+template <int CPL>
+__device__ __forceinline__ void sum_shares(float (&y)[CPL], const float* x, size_t step, int parts, float f) {
+  typedef __attribute__((ext_vector_type(CPL))) float fv;
+  for (int j = 0; j < parts; j += 8) {
+    fv v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = *reinterpret_cast<const fv*>(x + (size_t)min(j + u, parts - 1) * step);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float w = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(f), j + u));
+#pragma unroll
+      for (int c = 0; c < CPL; ++c) y[c] += v[u][c] * w;
+    }
+  }
+}
+
 // the same for few shares: a wave a row, HD / 64 columns a lane, four rows a workgroup
 template <int HD>
 __global__ __launch_bounds__(256) void attn_paged_merge_few_kernel(PagedArgs a) {
@@ -816,11 +833,7 @@ __global__ __launch_bounds__(256) void attn_paged_merge_few_kernel(PagedArgs a) 
   float y[CPL];
 #pragma unroll
   for (int c = 0; c < CPL; ++c) y[c] = 0.f;
-  for (int i = 0; i < parts; ++i) {
-    const float w = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(f), i));
-#pragma unroll
-    for (int c = 0; c < CPL; ++c) y[c] += po[(size_t)i * HD + c] * w;
-  }
+  sum_shares<CPL>(y, po, HD, parts, f);
   bf16_t* op = a.out + (size_t)t * a.ldo + (size_t)h * HD + lane * CPL;
   if (CPL == 2) *reinterpret_cast<unsigned*>(op) = pack2bf(y[0] * inv, y[CPL - 1] * inv);
   else *op = f2bf(y[0] * inv);
@@ -849,12 +862,7 @@ __global__ __launch_bounds__(256) void attn_paged_merge_tiles_kernel(PagedArgs a
     float y[CPL];
 #pragma unroll
     for (int c = 0; c < CPL; ++c) y[c] = 0.f;
-    for (int j = 0; j < parts; ++j) {
-      const float w = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(f), j));
-      const float* po = a.part_o + (p0 + j * step) * HD + lane * CPL;
-#pragma unroll
-      for (int c = 0; c < CPL; ++c) y[c] += po[c] * w;
-    }
+    sum_shares<CPL>(y, a.part_o + p0 * HD + lane * CPL, step * HD, parts, f);
     bf16_t* op = a.out + (size_t)t * a.ldo + (size_t)h * HD + lane * CPL;
     if (CPL == 2) *reinterpret_cast<unsigned*>(op) = pack2bf(y[0] * inv, y[CPL - 1] * inv);
     else *op = f2bf(y[0] * inv);
@@ -966,7 +974,7 @@ extern "C" int zk_attn_paged(const void* q, const void* k_cache, const void* v_c
   if (p.splits > 1 && p.mt == 8) {
     const int64_t wgs = (T * Hq + 3) / 4;
     void (*merge)(PagedArgs) = head_dim == 128 ? attn_paged_merge_tiles_kernel<128> : attn_paged_merge_tiles_kernel<64>;
-    hipLaunchKernelGGL(merge, dim3((unsigned)(wgs < 2048 ? wgs : 2048)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(merge, dim3((unsigned)(wgs < 8192 ? wgs : 8192)), dim3(256), 0, stream, a);
   } else if (p.splits > 1) {
     // few shares: a wave a row; many of few rows: four (two) workgroups a row
     const bool few = p.splits <= 16, slices = p.splits > 64 && T * Hq < 256;

@@ -12,6 +12,7 @@ from typing import Optional
 import torch
 
 import ctypes
+import functools
 
 from ._lib import GemmPlan, check, lib
 
@@ -284,29 +285,37 @@ def attn_decode_fused(qkv, cos_t, sin_t, k_cache, v_cache, pos: int, Hq: int, Hk
 
 def _here(name: str, *tensors):
     """The call's tensors are on the current device, where the kernel is launched (None passes)."""
-    dev = None
+    dev = -2
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError(f"{name}: zero_amd kernels need ROCm device tensors (no CPU path exists)")
-        if dev is None:
-            dev = torch.cuda.current_device()
-        if t.get_device() != dev:
-            raise ValueError(f"{name}: a tensor on cuda:{t.get_device()}, but the current device is cuda:{dev}")
+        if t is not None:
+            at = t.get_device()
+            if dev == -2:
+                dev = torch.cuda.current_device() if at >= 0 else -1
+            if at != dev or at < 0:
+                if at < 0:
+                    raise ValueError(f"{name}: zero_amd kernels need ROCm device tensors (no CPU path exists)")
+                raise ValueError(f"{name}: a tensor on cuda:{at}, but the current device is cuda:{dev}")
+
+
+def _rows2d(name: str, what: str, t, rows: int, width: int) -> int:
+    """Row stride of a bf16 row-major view [rows, width] (its device is checked by _here)."""
+    if t.dtype != BF16 or t.shape != (rows, width) or (t.stride(1) != 1 and width > 1):
+        raise ValueError(f"{name}: {what} must be a row-major bf16 view [{rows}, {width}], got {t.dtype} "
+                         f"{tuple(t.shape)} strides {t.stride()}")
+    return t.stride(0) if rows > 1 else (width + 7) // 8 * 8
 
 
 def _chk_paged_cache(name: str, k_cache, v_cache, width: int):
-    for t in (k_cache, v_cache):
-        if t.dtype != BF16 or t.dim() != 3 or t.shape[2] != width or not t.is_contiguous():
-            raise ValueError(f"{name}: caches must be contiguous bf16 [pages, page_size, Hkv*hd]")
-    if k_cache.shape != v_cache.shape:
-        raise ValueError(f"{name}: key and value caches differ in shape")
+    shape = k_cache.shape
+    if (k_cache.dtype != BF16 or v_cache.dtype != BF16 or len(shape) != 3 or shape[2] != width or v_cache.shape != shape
+            or not k_cache.is_contiguous() or not v_cache.is_contiguous()):
+        raise ValueError(f"{name}: key and value caches must be contiguous bf16 [pages, page_size, {width}] of one shape")
+    return shape
 
 
-def _chk_i32(name: str, t, n: int, what: str):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
-        raise ValueError(f"{name}: {what} must be contiguous int32 [{n}]")
+def _chk_vec(name: str, t, n: int, dtype, what: str):
+    if t.dtype != dtype or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name}: {what} must be contiguous {dtype} [{n}]")
 
 
 def kv_append_paged(qkv, cos_t, sin_t, k_cache, v_cache, positions, slots, Hq: int, Hkv: int, hd: int,
@@ -319,31 +328,31 @@ def kv_append_paged(qkv, cos_t, sin_t, k_cache, v_cache, positions, slots, Hq: i
     Caches: contiguous [pages, page_size, Hkv*hd]; the live slots of one call are distinct."""
     name = "kv_append_paged"
     _here(name, qkv, cos_t, sin_t, k_cache, v_cache, positions, slots, q_out)
-    _chk2d(qkv, "qkv")
     T = qkv.shape[0]
-    if Hq <= 0 or Hkv <= 0 or Hq % Hkv or qkv.shape[1] != (Hq + 2 * Hkv) * hd:
-        raise ValueError(f"{name}: qkv must be [T, (Hq + 2 Hkv) * hd]")
-    _chk_paged_cache(name, k_cache, v_cache, Hkv * hd)
-    if (cos_t.dtype != torch.float32 or cos_t.dim() != 2 or not cos_t.is_contiguous() or sin_t.dtype != torch.float32
-            or sin_t.shape != cos_t.shape or not sin_t.is_contiguous()):
+    if Hq <= 0 or Hkv <= 0 or Hq % Hkv:
+        raise ValueError(f"{name}: Hq must be a multiple of Hkv")
+    ldqkv = _rows2d(name, "qkv", qkv, T, (Hq + 2 * Hkv) * hd)
+    pages, page, _ = _chk_paged_cache(name, k_cache, v_cache, Hkv * hd)
+    table = cos_t.shape
+    if (cos_t.dtype != torch.float32 or len(table) != 2 or not cos_t.is_contiguous() or sin_t.dtype != torch.float32
+            or sin_t.shape != table or not sin_t.is_contiguous()):
         raise ValueError(f"{name}: cos / sin tables must be contiguous fp32 [positions, rot / 2]")
-    _chk_i32(name, positions, T, "positions"); _chk_i32(name, slots, T, "slots")
+    _chk_vec(name, positions, T, torch.int32, "positions")
+    _chk_vec(name, slots, T, torch.int32, "slots")
     if q_out is None:
-        q_out = torch.empty((T, Hq * hd), dtype=BF16, device=qkv.device)
-    else:
-        _chk2d(q_out, "q_out")
-        if q_out.shape != (T, Hq * hd):
-            raise ValueError(f"{name}: q_out must be [T, Hq * hd]")
+        q_out = qkv.new_empty((T, Hq * hd))
+    ldq = _rows2d(name, "q_out", q_out, T, Hq * hd)
     if T == 0:
         return q_out
-    rows, half = cos_t.shape
-    check(lib.zk_kv_append_paged(qkv.data_ptr(), cos_t.data_ptr(), sin_t.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(),
-                                 v_cache.data_ptr(), positions.data_ptr(), slots.data_ptr(), T, Hq, Hkv, hd, 2 * half, rows,
-                                 _ld(qkv), _ld(q_out), k_cache.shape[0] * k_cache.shape[1], int(interleaved), _stream()),
-          "zk_kv_append_paged")
+    rc = lib.zk_kv_append_paged(qkv.data_ptr(), cos_t.data_ptr(), sin_t.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(),
+                                v_cache.data_ptr(), positions.data_ptr(), slots.data_ptr(), T, Hq, Hkv, hd, 2 * table[1],
+                                table[0], ldqkv, ldq, pages * page, 1 if interleaved else 0, _stream())
+    if rc:
+        check(rc, name)
     return q_out
 
 
+@functools.lru_cache(maxsize=256)
 def attn_paged_ws_floats(B: int, T: int, max_q: int, max_ctx: int, Hq: int, Hkv: int, hd: int) -> int:
     """fp32 values of workspace that attn_paged needs for such a call."""
     n = ctypes.c_int64()
@@ -363,26 +372,24 @@ def attn_paged(q, k_cache, v_cache, page_table, ctx_lens, cu_q, max_q: int, max_
     ws: fp32 workspace of at least attn_paged_ws_floats(...) values (allocated when not given)."""
     name = "attn_paged"
     _here(name, q, k_cache, v_cache, page_table, ctx_lens, cu_q, tree_mask, out, ws)
-    _chk2d(q, "q")
     T = q.shape[0]
-    if Hq <= 0 or Hkv <= 0 or Hq % Hkv or q.shape[1] != Hq * hd:
-        raise ValueError(f"{name}: q must be [T, Hq * hd] with Hq a multiple of Hkv")
-    _chk_paged_cache(name, k_cache, v_cache, Hkv * hd)
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1:
+    if Hq <= 0 or Hkv <= 0 or Hq % Hkv:
+        raise ValueError(f"{name}: Hq must be a multiple of Hkv")
+    ldq = _rows2d(name, "q", q, T, Hq * hd)
+    pages, page, _ = _chk_paged_cache(name, k_cache, v_cache, Hkv * hd)
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
         raise ValueError(f"{name}: page_table must be int32 [B, columns]")
     B, cols = page_table.shape
-    _chk_i32(name, ctx_lens, B, "ctx_lens"); _chk_i32(name, cu_q, B + 1, "cu_q")
-    words = 0
+    _chk_vec(name, ctx_lens, B, torch.int32, "ctx_lens")
+    _chk_vec(name, cu_q, B + 1, torch.int32, "cu_q")
+    words, mask = 0, None
     if tree_mask is not None:
         if tree_mask.dtype != torch.int64 or tree_mask.dim() != 2 or tree_mask.shape[0] != T or not tree_mask.is_contiguous():
             raise ValueError(f"{name}: tree_mask must be contiguous int64 [T, words]")
-        words = tree_mask.shape[1]
+        words, mask = tree_mask.shape[1], tree_mask.data_ptr()
     if out is None:
-        out = torch.empty((T, Hq * hd), dtype=BF16, device=q.device)
-    else:
-        _chk2d(out, "out")
-        if out.shape != (T, Hq * hd):
-            raise ValueError(f"{name}: out must be [T, Hq * hd]")
+        out = q.new_empty((T, Hq * hd))
+    ldo = _rows2d(name, "out", out, T, Hq * hd)
     need = attn_paged_ws_floats(B, T, max_q, max_ctx, Hq, Hkv, hd)
     if ws is None:
         if need:
@@ -391,10 +398,12 @@ def attn_paged(q, k_cache, v_cache, page_table, ctx_lens, cu_q, max_q: int, max_
         raise ValueError(f"{name}: ws must be contiguous fp32 with at least {need} values")
     if T == 0:
         return out
-    check(lib.zk_attn_paged(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), page_table.data_ptr(),
-                            ctx_lens.data_ptr(), cu_q.data_ptr(), _p(tree_mask), _p(ws), ws.numel() if ws is not None else 0,
-                            T, B, max_q, max_ctx, Hq, Hkv, hd, k_cache.shape[1], k_cache.shape[0], cols, _ld(page_table),
-                            words, _ld(q), _ld(out), scale, _stream()), "zk_attn_paged")
+    rc = lib.zk_attn_paged(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), page_table.data_ptr(),
+                           ctx_lens.data_ptr(), cu_q.data_ptr(), mask, ws.data_ptr() if need else None, need, T, B, max_q,
+                           max_ctx, Hq, Hkv, hd, page, pages, cols, page_table.stride(0) if B > 1 else cols, words, ldq, ldo,
+                           scale, _stream())
+    if rc:
+        check(rc, name)
     return out
 
 
@@ -407,26 +416,37 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     the token drawn is the first whose running sum exceeds u times the kept sum (64-bit sums).  -inf is never drawn; a row
     of -inf gives token -1 with -inf, a row with a NaN -1 with NaN."""
     name = "sample"
-    rows_of = [v if torch.is_tensor(v) else None for v in (temperature, top_k, top_p, min_p)]
-    _here(name, logits, u, *rows_of)
-    _chk2d(logits, "logits")
+    t, k, p, mp = temperature, top_k, top_p, min_p
+    tt, kt, pt, mt = (v if torch.is_tensor(v) else None for v in (t, k, p, mp))
+    _here(name, logits, u, tt, kt, pt, mt)
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError(f"{name}: logits must be [rows, vocabulary]")
     rows, V = logits.shape
-    if V == 0:
-        raise ValueError(f"{name}: empty vocabulary")
-    for t, n, d in zip([u] + rows_of, ("u", "temperature", "top_k", "top_p", "min_p"),
-                       (torch.float32, torch.float32, torch.int32, torch.float32, torch.float32)):
-        if t is not None and (t.dtype != d or t.dim() != 1 or t.shape[0] != rows or (rows > 1 and t.stride(0) != 1)):
-            raise ValueError(f"{name}: {n} must be a contiguous {d} tensor [{rows}]")
-    t, k, p, mp = (0 if r is not None else v for r, v in zip(rows_of, (temperature, top_k, top_p, min_p)))
-    if ((rows_of[0] is None and not 0 <= t <= 2 ** 20) or (rows_of[1] is None and not (0 <= k < 2 ** 31 and k == int(k)))
-            or (rows_of[2] is None and not 0 < p <= 1) or (rows_of[3] is None and not 0 <= mp <= 1)):
+    if logits.dtype != BF16 or (logits.stride(1) != 1 and V > 1):
+        raise ValueError(f"{name}: logits must be a row-major bf16 view")
+    _chk_vec(name, u, rows, torch.float32, "u")
+    if tt is not None:
+        t = 0.0
+        _chk_vec(name, tt, rows, torch.float32, "temperature")
+    if kt is not None:
+        k = 0
+        _chk_vec(name, kt, rows, torch.int32, "top_k")
+    if pt is not None:
+        p = 1.0
+        _chk_vec(name, pt, rows, torch.float32, "top_p")
+    if mt is not None:
+        mp = 0.0
+        _chk_vec(name, mt, rows, torch.float32, "min_p")
+    if not (0 <= t <= 2 ** 20 and 0 <= k < 2 ** 31 and k == int(k) and 0 < p <= 1 and 0 <= mp <= 1):
         raise ValueError(f"{name}: temperature in [0, 2^20], top_k a whole number >= 0, top_p in (0, 1], min_p in [0, 1]")
     tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
-    logp = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    logp = u.new_empty((rows,))
     if rows == 0:
         return tokens, logp
-    check(lib.zk_sample(logits.data_ptr(), u.data_ptr(), _p(rows_of[0]), _p(rows_of[1]), _p(rows_of[2]), _p(rows_of[3]),
-                        t, int(k), p, mp, tokens.data_ptr(), logp.data_ptr(), rows, V, _ld(logits), _stream()), "zk_sample")
+    rc = lib.zk_sample(logits.data_ptr(), u.data_ptr(), _p(tt), _p(kt), _p(pt), _p(mt), t, int(k), p, mp, tokens.data_ptr(),
+                       logp.data_ptr(), rows, V, logits.stride(0) if rows > 1 else V, _stream())
+    if rc:
+        check(rc, name)
     return tokens, logp
 
 
