@@ -289,3 +289,175 @@ def test_decode_step_of_the_three_operators_in_a_captured_graph():
         assert torch.equal(kv, other)
         for a, b in zip(held, want):
             assert torch.equal(a, b), i
+
+
+@pytest.mark.parametrize("Hq,Hkv,hd,page", [(8, 2, 128, 64), (16, 2, 64, 128), (6, 1, 128, 48)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_attn_paged_shares_of_long_ragged_sequences(Hq, Hkv, hd, page, tree):
+    """Many-row tiles whose keys are dealt out over workgroups by the sequences' own lengths, and merged."""
+    c = make([(37, 3001), (70, 700), (9, 20), (0, 90), (41, 41), (33, 1999)], Hq, Hkv, hd, page, tree=tree, seed=21)
+    agree(call(c), c)
+
+
+@pytest.mark.parametrize("ctx", [5000, 40001])
+@pytest.mark.parametrize("Hq,Hkv,hd", [(8, 1, 128), (4, 2, 64), (40, 2, 128)])
+def test_attn_paged_single_tokens_far_into_the_cache(ctx, Hq, Hkv, hd):
+    c = make([(1, ctx), (1, 300)], Hq, Hkv, hd, 64, seed=22, poison=False)
+    agree(call(c), c)
+
+
+def test_attn_paged_more_sequences_than_lanes():
+    """150 sequences, some without new tokens: the layout of shares is found over several rounds of 64."""
+    rng = random.Random(1)
+    seqs = [(rng.choice([0, 1, 3, 20, 34]), 0) for _ in range(150)]
+    seqs = [(n, n + rng.randrange(0, 330)) for n, _ in seqs]
+    c = make(seqs, 4, 2, 64, 16, seed=23)
+    agree(call(c), c)
+
+
+def differ_like(got, want, mag):
+    """Where the formula is finite: as ``agree``; where it is infinite or NaN: the same."""
+    got = got.double().cpu()
+    fin = torch.isfinite(want)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    inf = torch.isinf(want)
+    assert torch.equal(got[inf], want[inf])
+    tol = HALF_STEP * want.abs() + (HALF_STEP + 2.0 ** -11) * mag + 1e-30
+    assert ((got - want).abs()[fin] <= tol[fin]).all()
+
+
+@pytest.mark.parametrize("seqs", [[(1, 40), (3, 9)], [(8, 50), (5, 5)], [(40, 130), (70, 70)]], ids=["few", "some", "many"])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("tree", [False, True])
+def test_attn_paged_infinities_and_nan_reach_those_that_see_them_only(seqs, page, tree):
+    """New rows whose values hold infinities or NaN, seen by later tokens (or a branch) and hidden from the others."""
+    Hq, Hkv, hd = 8, 2, 128
+    c = make(seqs, Hq, Hkv, hd, page, tree=tree, seed=31)
+    for b, (n, ctx) in enumerate(seqs):
+        for j, val in ((n // 3, math.inf), (n // 2, math.nan), (n - 1, -math.inf)):
+            r = ctx - n + j
+            c["v"][int(c["table"][b, r // page]), r % page, 5 + j % 3::17] = val
+    want, mag = ref.attention(c["q"], c["k"], c["v"], c["table"], c["ctx"], c["cu"], Hq, Hkv, hd, hd ** -0.5, c["mask"])
+    differ_like(call(c), want, torch.nan_to_num(mag, nan=0.0, posinf=0.0))
+
+
+def test_attn_paged_nan_keys_reach_those_that_see_them_only():
+    c = make([(40, 100), (1, 7)], 8, 2, 128, 64, seed=32)
+    c["k"][int(c["table"][0, 80 // 64]), 80 % 64, 3] = math.nan        # key 80 = new token 20, head 0
+    want, mag = ref.attention(c["q"], c["k"], c["v"], c["table"], c["ctx"], c["cu"], 8, 2, 128, 128 ** -0.5)
+    assert want[:20].isfinite().all() and want[20:40, :4 * 128].isnan().all()
+    differ_like(call(c), want, torch.nan_to_num(mag))
+
+
+def test_attn_paged_bounds_from_the_host_only_shape_the_launch():
+    """max_q and max_ctx larger than needed (a captured graph's bounds) give the same answer within the tolerance, max_ctx
+    smaller than a length too; tokens past max_q are left as they are."""
+    from zero_amd import ops
+    c = make([(2, 500), (1, 33)], 8, 2, 128, 16, seed=33)
+    d = {k: (v.to(DEV) if torch.is_tensor(v) else v) for k, v in c.items()}
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+
+    def run(max_q, max_ctx, out=None):
+        return ops.attn_paged(d["q"], d["k"], d["v"], d["table"], i32(c["ctx"]), i32(c["cu"]), max_q, max_ctx, 8, 2, 128,
+                              128 ** -0.5, out=out)
+    for max_q, max_ctx in ((2, 500), (2, 40), (7, 3000), (30, 100000), (30, 300)):
+        agree(run(max_q, max_ctx), c)
+    out = torch.full_like(d["q"], 9.0)
+    run(1, 500, out)
+    assert (out[1] == 9).all() and not (out[0] == 9).all() and not (out[2] == 9).all()
+
+
+def test_operators_on_a_side_stream_and_two_at_once():
+    """Inputs made on one stream and used on another that waited for it; two streams at the same time, a workspace each."""
+    from zero_amd import ops
+    cs = [make([(1, 3000), (20, 900)], 8, 2, 128, 64, seed=s) for s in (41, 42)]
+    want = [call(c) for c in cs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(3):
+        got.clear()
+        for c, st in zip(cs, streams):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                got.append(call(c))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    x = torch.randn(5, 70000, device=DEV).to(BF16)
+    u = torch.rand(5, device=DEV)
+    a = ops.sample(x, u)
+    streams[0].wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(streams[0]):
+        b = ops.sample(x, u)
+    torch.cuda.synchronize()
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_two_captured_graphs_with_a_workspace_each():
+    """Two graphs of shared-out attention, replayed in turn and overlapping on two streams."""
+    from zero_amd import ops
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    graphs, outs, want, alive = [], [], [], []                  # a graph reads its inputs where they lay at capture
+    for s in (51, 52):
+        c = make([(20, 1500), (1, 700)], 8, 2, 128, 64, seed=s)
+        d = {k: (v.to(DEV) if torch.is_tensor(v) else v) for k, v in c.items()}
+        ws = torch.empty(max(1, ops.attn_paged_ws_floats(2, 21, 20, 1500, 8, 2, 128)), device=DEV)
+        ctx, cu = i32(c["ctx"]), i32(c["cu"])
+        f = lambda d=d, ws=ws, ctx=ctx, cu=cu: ops.attn_paged(d["q"], d["k"], d["v"], d["table"], ctx, cu, 20, 1500, 8, 2,  # noqa: E731
+                                                              128, 128 ** -0.5, ws=ws)
+        alive.append((d, ws, ctx, cu))
+        want.append(f().clone())
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(f())
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(4):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o, w)
+            o.zero_()
+        torch.cuda.synchronize()
+
+
+def test_wrapper_refusals_on_the_device():
+    from zero_amd import ops
+    c = make([(2, 20)], 4, 2, 64, 16)
+    d = {k: (v.to(DEV) if torch.is_tensor(v) else v) for k, v in c.items()}
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    ok = dict(q=d["q"], k_cache=d["k"], v_cache=d["v"], page_table=d["table"], ctx_lens=i32([20]), cu_q=i32([0, 2]), max_q=2,
+              max_ctx=20, Hq=4, Hkv=2, hd=64, scale=0.1)
+    ops.attn_paged(**ok)
+    for bad in (dict(q=d["q"].float()), dict(q=d["q"][:, :128]), dict(Hkv=3), dict(k_cache=d["k"][:, ::2]),
+                dict(v_cache=d["v"][:2]), dict(page_table=d["table"].long()), dict(ctx_lens=i32([20, 3])), dict(cu_q=i32([0])),
+                dict(ctx_lens=d["q"][:1, 0]), dict(tree_mask=torch.zeros(3, 1, dtype=torch.int64, device=DEV)),
+                dict(tree_mask=torch.zeros(2, 1, dtype=torch.int32, device=DEV)), dict(out=torch.empty(2, 64, device=DEV)),
+                dict(ctx_lens=torch.tensor([20], dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            ops.attn_paged(**{**ok, **bad})
+    from zero_amd._lib import ZeroHipError
+    with pytest.raises((ValueError, ZeroHipError)):
+        ops.attn_paged(**{**ok, "max_q": 0})
+    qkv = torch.zeros((2, 8 * 64), dtype=BF16, device=DEV)
+    cos = torch.ones((4, 32), device=DEV)
+    ok = dict(qkv=qkv, cos_t=cos, sin_t=cos, k_cache=d["k"], v_cache=d["v"], positions=i32([0, 1]), slots=i32([-1, -1]), Hq=4,
+              Hkv=2, hd=64)
+    ops.kv_append_paged(**ok)
+    for bad in (dict(qkv=qkv[:, :256]), dict(cos_t=cos.double()), dict(sin_t=cos[:2]), dict(positions=i32([0])),
+                dict(slots=i32([0, 1]).long()), dict(k_cache=d["k"].view(-1, 128)), dict(q_out=qkv)):
+        with pytest.raises(ValueError):
+            ops.kv_append_paged(**{**ok, **bad})
+    for half in (4, 48):                                       # 8 values are no whole unit, 96 more than the head
+        t = torch.ones((4, half), device=DEV)
+        with pytest.raises(ZeroHipError):
+            ops.kv_append_paged(**{**ok, "cos_t": t, "sin_t": t})
+    x, u = torch.zeros((2, 9), dtype=BF16, device=DEV), torch.zeros(2, device=DEV)
+    ops.sample(x, u)
+    for bad in (dict(logits=x.float()), dict(logits=x.t()), dict(u=u[:1]), dict(u=u.double()), dict(temperature=-1.0),
+                dict(temperature=math.nan), dict(top_k=-1), dict(top_k=1.5), dict(top_p=0.0), dict(top_p=1.1), dict(min_p=2.0),
+                dict(temperature=u.double()), dict(top_k=u), dict(top_p=u[:1]), dict(u=u.cpu())):
+        with pytest.raises(ValueError):
+            ops.sample(**{**dict(logits=x, u=u), **bad})
