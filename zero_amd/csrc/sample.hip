@@ -342,19 +342,30 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     if (!RESIDENT) { x.load(row, part, left(part), skew, tid); x.to_keys(left(part)); }
     typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      int n = 0;
-      if (c * kThreads * 8 < left(part)) {
-        u16x2 other = {0, 0};                       // halves that differ
+    for (int c4 = 0; c4 < kChunks; c4 += 4) {       // most groups of chunks hold no match: one test for four
+      int mine[4] = {0, 0, 0, 0};
+      if (c4 * kThreads * 8 < left(part)) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const unsigned w = x.r[c][e] ^ key2;
-          other += __builtin_elementwise_min(__builtin_bit_cast(u16x2, w), (u16x2){1, 1});
+        for (int k = 0; k < 4; ++k) {
+          u16x2 other = {0, 0};                     // halves that differ: min(x ^ key, 1), one packed instruction in
+#pragma unroll                                      // place of the compiler's compare and select for each half
+          for (int e = 0; e < 4; ++e) {
+            unsigned w;
+            asm("v_pk_min_u16 %0, %1, 1 op_sel_hi:[1,0]" : "=v"(w) : "v"(x.r[c4 + k][e] ^ key2));
+            other += __builtin_bit_cast(u16x2, w);
+          }
+          const unsigned sum = __builtin_bit_cast(unsigned, other);
+          mine[k] = 8 - (int)((sum & 0xFFFFu) + (sum >> 16));
         }
-        const int mine = 8 - (int)other[0] - (int)other[1];
-        if (__any(mine)) n = lane_of(wave_upto(mine), 63);
+        if (__any(mine[0] | mine[1] | mine[2] | mine[3])) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mine[k] = wave_upto(mine[k]);
+        }
       }
-      if (lane == 0) matches[c * kWaves + wave] = (unsigned)n;
+      if (lane == 63) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) matches[(c4 + k) * kWaves + wave] = (unsigned)mine[k];
+      }
     }
     __syncthreads();
     const u32x4 m4 = *reinterpret_cast<const u32x4*>(&matches[lane * 4]);
