@@ -91,6 +91,35 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
+// inclusive sum over the wave's lanes in DPP steps (rows of 16, then their ends broadcast): no LDS round trips
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp0(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp0(double v) {
+  return __hiloint2double(dpp0<CTRL, ROWS>(__double2hiint(v)), dpp0<CTRL, ROWS>(__double2loint(v)));
+}
+template <class T>
+__device__ __forceinline__ T wave_upto(T v) {
+  v += dpp0<0x111, 0xF>(v);
+  v += dpp0<0x112, 0xF>(v);
+  v += dpp0<0x114, 0xF>(v);
+  v += dpp0<0x118, 0xF>(v);
+  v += dpp0<0x142, 0xA>(v);
+  v += dpp0<0x143, 0xC>(v);
+  return v;
+}
+// largest over the wave, in DPP steps; the same in all lanes
+__device__ __forceinline__ int wave_top(int v) {
+  const int low = (int)0x80000000;
+  v = max(v, __builtin_amdgcn_update_dpp(low, v, 0x111, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(low, v, 0x112, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(low, v, 0x114, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(low, v, 0x118, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(low, v, 0x142, 0xA, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(low, v, 0x143, 0xC, 0xF, false));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
 // 16-byte global load through a buffer descriptor; out-of-range offsets return 0.
 __device__ __forceinline__ u32x4 buf_load16(__amdgpu_buffer_rsrc_t r, unsigned int byte_off) {
   return __builtin_amdgcn_raw_buffer_load_b128(r, byte_off, 0, 0);

@@ -197,11 +197,10 @@ struct Shares {
     for (int b0 = 0; b0 < a.B; b0 += 64) {
       of(a, b0 + lane, tiles, len);
       all += tiles;
-      longest = max(longest, tiles ? len : 1);
+      longest = max(longest, tiles ? len : 1);      // (B <= 64: the lanes keep their sequence's)
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) { all += __shfl_xor(all, o, 64); longest = max(longest, __shfl_xor(longest, o, 64)); }
-    all *= a.Hkv;
+    all = __builtin_amdgcn_readlane(wave_upto(all), 63) * a.Hkv;
+    longest = wave_top(longest);
     q = longest;
     if (a.part_o && longest > 4 && all < 2 * slots) {
       const int mine = (longest + lane) / (lane + 1);
@@ -215,9 +214,7 @@ struct Shares {
       n *= a.Hkv;
       int cost = (n + slots - 1) / slots * (mine + 4);
       if (n > 2 * slots && lane) cost = 0x1FFFFFF;
-      int best = (min(cost, 0x1FFFFFF) << 6) | lane;
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) best = min(best, __shfl_xor(best, o, 64));
+      const int best = -wave_top(-((min(cost, 0x1FFFFFF) << 6) | lane));
       q = (longest + (best & 63)) / ((best & 63) + 1);
     }
     for (;;) {
@@ -226,12 +223,7 @@ struct Shares {
       for (int b0 = 0; b0 < a.B; b0 += 64) {
         if (a.B > 64) of(a, b0 + lane, tiles, len);
         const int u = a.Hkv * ((len + q - 1) / q), n = tiles * u;
-        int upto = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-          const int y = __shfl_up(upto, o, 64);
-          if (lane >= o) upto += y;
-        }
+        const int upto = wave_upto(n);
         const int start = before + upto - n;
         if (id == 0 && threadIdx.x < 64 && a.part_o && b0 + lane < a.B) a.shares[1 + b0 + lane] = start;
         const unsigned long long hit = __ballot(id >= start && id < start + n);

@@ -90,23 +90,6 @@ struct Row {
   }
 };
 
-// inclusive sum over the wave's lanes in DPP steps (rows of 16, then their ends broadcast): no LDS round trips
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp0(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true); }
-template <int CTRL, int ROWS>
-__device__ __forceinline__ double dpp0(double v) {
-  return __hiloint2double(dpp0<CTRL, ROWS>(__double2hiint(v)), dpp0<CTRL, ROWS>(__double2loint(v)));
-}
-template <class T>
-__device__ __forceinline__ T wave_upto(T v) {
-  v += dpp0<0x111, 0xF>(v);
-  v += dpp0<0x112, 0xF>(v);
-  v += dpp0<0x114, 0xF>(v);
-  v += dpp0<0x118, 0xF>(v);
-  v += dpp0<0x142, 0xA>(v);
-  v += dpp0<0x143, 0xC>(v);
-  return v;
-}
 __device__ __forceinline__ double lane_of(double v, int lane) {     // lane: the same in the whole wave
   return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane), __builtin_amdgcn_readlane(__double2loint(v), lane));
 }
