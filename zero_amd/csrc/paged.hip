@@ -553,26 +553,29 @@ __global__ __launch_bounds__(256, kTileSlots<HD> / 256) void attn_paged_tile_ker
 
   int row, next = -1;                               // cache row of key `lane` (ONE_PAGE: of the first key) of a tile
   auto look = [&](int t) __attribute__((always_inline)) { return cache_row(a, b, ks + t * KV + (ONE_PAGE ? 0 : lane), ke); };
-  auto issue = [&](int t, int rr) __attribute__((always_inline)) {
-    unsigned char* st = smem + (t & 1) * STAGE;
-    const size_t tile0 = ONE_PAGE ? (size_t)max(__builtin_amdgcn_readfirstlane(rr), 0) * kvw : 0;
+  // A tile's DMA in 2 NQ pieces (16 bytes a lane; even: K, odd: V).  Behind the barrier they go out one between the
+  // matrix instructions of each k-step: in a burst each holds its wave for 60 to 180 cycles.
+  size_t from[ONE_PAGE ? 1 : NQ];
+  auto aim = [&](int rr) __attribute__((always_inline)) {
+    if (ONE_PAGE) {
+      from[0] = (size_t)max(__builtin_amdgcn_readfirstlane(rr), 0) * kvw;
+    } else {
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-      const int sidx = tid + 256 * i, trow = sidx / CPR, ch = (sidx % CPR) ^ swz_key<HD>(trow);
-      const size_t off = ONE_PAGE ? (size_t)(unsigned)(trow * kvw + ch * 8) : (size_t)max(__shfl(rr, trow, 64), 0) * kvw + ch * 8;
-      unsigned char* dst = st + (wave * 64 + 256 * i) * 16;
-      if (ONE_PAGE) {
-        lds_dma_at(dst, kb + tile0, (unsigned)(off * 2));
-        lds_dma_at(dst + TB, vb + tile0, (unsigned)(off * 2));
-      } else {
-        lds_dma_from(dst, kb + off);
-        lds_dma_from(dst + TB, vb + off);
-      }
+      for (int i = 0; i < NQ; ++i) from[i] = (size_t)max(__shfl(rr, (tid + 256 * i) / CPR, 64), 0) * kvw;
     }
+  };
+  auto piece = [&](int t, int i2) __attribute__((always_inline)) {
+    const int i = i2 >> 1, sidx = tid + 256 * i, trow = sidx / CPR, ch = (sidx % CPR) ^ swz_key<HD>(trow);
+    unsigned char* dst = smem + (t & 1) * STAGE + (i2 & 1) * TB + (wave * 64 + 256 * i) * 16;
+    const bf16_t* src = i2 & 1 ? vb : kb;
+    if (ONE_PAGE) lds_dma_at(dst, src + from[0], (unsigned)(trow * kvw + ch * 8) * 2u);
+    else lds_dma_from(dst, src + from[ONE_PAGE ? 0 : i] + ch * 8);
   };
   row = look(0);
   if (nt > 0) {
-    issue(0, row);
+    aim(row);
+#pragma unroll
+    for (int i = 0; i < 2 * NQ; ++i) piece(0, i);
     next = look(1);
   }
   bf16x8 qf[C::DS];
@@ -600,8 +603,9 @@ __global__ __launch_bounds__(256, kTileSlots<HD> / 256) void attn_paged_tile_ker
     unsigned char* kl = smem + (t & 1) * STAGE;
     unsigned char* vl = kl + TB;
     row = next;
-    if (t + 1 < nt) {
-      issue(t + 1, row);
+    const bool more = t + 1 < nt;
+    if (more) {
+      aim(row);
       next = look(t + 2);
     }
     const bool edge = k0 + KV > clear || ok != ~0ull;        // uniform over the workgroup: some row may not see some key
@@ -624,14 +628,29 @@ __global__ __launch_bounds__(256, kTileSlots<HD> / 256) void attn_paged_tile_ker
     }
     f32x16 st[2];
     const bool wanted = k0 < last_wave;
+    if (!wanted && more) {
+#pragma unroll
+      for (int i = 0; i < 2 * NQ; ++i) piece(t + 1, i);
+    }
     if (wanted) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int e = 0; e < 16; ++e) st[x][e] = 0.f;
+      // fragments of the next k-step are requested ahead of a step's matrix instructions and its piece of DMA (2 NQ = DS)
+      static_assert(2 * NQ == C::DS, "a piece a k-step");
+      bf16x8 kf[2][2];
 #pragma unroll
-        for (int ds = 0; ds < C::DS; ++ds)
-          st[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag_sw<HD>(kl, x * 32, ds, lane), qf[ds], st[x], 0, 0, 0);
+      for (int x = 0; x < 2; ++x) kf[0][x] = row_frag_sw<HD>(kl, x * 32, 0, lane);
+#pragma unroll
+      for (int ds = 0; ds < C::DS; ++ds) {
+        if (ds + 1 < C::DS) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) kf[(ds + 1) & 1][x] = row_frag_sw<HD>(kl, x * 32, ds + 1, lane);
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) st[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ds & 1][x], qf[ds], st[x], 0, 0, 0);
+        if (more) piece(t + 1, ds);
       }
       if (__builtin_expect(edge, 0)) {
 #pragma unroll
