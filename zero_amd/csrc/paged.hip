@@ -107,6 +107,17 @@ struct PagedArgs {
 
 constexpr int kMaxRows = 1 << 30;
 
+// the larger of a value and that of the lane 16 / 32 away, without LDS (v_permlane{16,32}_swap of a value with itself
+// leaves the even halves in one register and the odd ones in the other)
+__device__ __forceinline__ float max_over16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_over32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 // one sequence's share of the call
 struct Seq {
   int q0, n, len;               // first row of q, new tokens, cached rows
@@ -350,8 +361,7 @@ __global__ __launch_bounds__(256, MT == 1 && HD == 64 ? 4 : 2) void attn_paged_s
       float mx = sc4[mt][0][0];
 #pragma unroll
       for (int e = 1; e < 8; ++e) mx = fmaxf(mx, sc4[mt][e >> 2][e & 3]);
-      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      mx = max_over32(max_over16(mx));
       mx *= sc;
       if (__any(mx > m[mt] + kSlack)) {
         const float mn = fmaxf(m[mt], mx), f = fast_exp2(m[mt] - (mn == -INFINITY ? 0.f : mn));
@@ -663,7 +673,7 @@ __global__ __launch_bounds__(256, kTileSlots<HD> / 256) void attn_paged_tile_ker
       float mx = fmaxf(st[0][0], st[1][0]);
 #pragma unroll
       for (int e = 1; e < 16; ++e) mx = fmaxf(mx, fmaxf(st[0][e], st[1][e]));
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * sc;
+      mx = max_over32(mx) * sc;
       if (__any(mx > m_run + kSlack)) {
         const float mn = fmaxf(m_run, mx), f = fast_exp2(m_run - (mn == -INFINITY ? 0.f : mn));
         l_run *= f;
