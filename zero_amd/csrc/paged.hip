@@ -637,6 +637,7 @@ __global__ __launch_bounds__(256, kTileSlots<HD> / 256) void attn_paged_tile_ker
             (unsigned)__builtin_amdgcn_readfirstlane((int)bad[0]);
     }
     f32x16 st[2];
+    float use = 0.f;
     const bool wanted = k0 < last_wave;
     if (!wanted && more) {
 #pragma unroll
@@ -681,17 +682,7 @@ __global__ __launch_bounds__(256, kTileSlots<HD> / 256) void attn_paged_tile_ker
 #pragma unroll
         for (int d = 0; d < C::DB; ++d) o[d] = o[d] * f;
       }
-      const float use = m_run == -INFINITY ? 0.f : m_run;
-      float rs = 0.f;
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p = fast_exp2(__builtin_fmaf(st[x][e], sc, -use));
-          st[x][e] = p;
-          rs += p;
-        }
-      l_run += rs;
+      use = m_run == -INFINITY ? 0.f : m_run;
     }
     if (__builtin_expect(odd != 0, 0)) {
       // keys with infinities or NaN in V: added on their own to the rows that see them, then zeros for the product below
@@ -703,7 +694,7 @@ __global__ __launch_bounds__(256, kTileSlots<HD> / 256) void attn_paged_tile_ker
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (e == (kk >> 5) * 16 + (kk & 3) + 4 * ((kk & 31) >> 3)) x = st[e >> 4][e & 15];
-          x = __shfl(x, ((kk >> 2) & 1) * 32 + (lane & 31), 64);
+          x = fast_exp2(__builtin_fmaf(__shfl(x, ((kk >> 2) & 1) * 32 + (lane & 31), 64), sc, -use));
           if (x != 0.f) {
 #pragma unroll
             for (int d = 0; d < C::DB; ++d)
@@ -723,15 +714,24 @@ __global__ __launch_bounds__(256, kTileSlots<HD> / 256) void attn_paged_tile_ker
       __syncthreads();
     }
     if (wanted) {
+      // 16 keys at a time: their exponentials, then the matrix instructions that take them
+      float rs = 0.f;
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
-          const bf16x8 pf = pack_acc(st[x], z);
+          bf16x8 pf;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float p = fast_exp2(__builtin_fmaf(st[x][8 * z + e], sc, -use));
+            pf[e] = (__bf16)p;                      // rounded to bf16 for the matrix product only
+            rs += p;
+          }
 #pragma unroll
           for (int d = 0; d < C::DB; ++d)
             o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_frag_sw<HD>(vl, x * 32, z, d, lane), pf, o[d], 0, 0, 0);
         }
+      l_run += rs;
     }
   }
   const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
