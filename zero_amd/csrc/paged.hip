@@ -714,7 +714,9 @@ __global__ __launch_bounds__(256, kTileSlots<HD> / 256) void attn_paged_tile_ker
       __syncthreads();
     }
     if (wanted) {
-      // 16 keys at a time: their exponentials, then the matrix instructions that take them
+      // 16 keys at a time: their exponentials, then the matrix instructions that take them; ahead of the co-resident
+      // workgroups' other phases (1 to 3 % at three workgroups a CU)
+      __builtin_amdgcn_s_setprio(1);
       float rs = 0.f;
 #pragma unroll
       for (int x = 0; x < 2; ++x)
@@ -732,6 +734,7 @@ __global__ __launch_bounds__(256, kTileSlots<HD> / 256) void attn_paged_tile_ker
             o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_frag_sw<HD>(vl, x * 32, z, d, lane), pf, o[d], 0, 0, 0);
         }
       l_run += rs;
+      __builtin_amdgcn_s_setprio(0);
     }
   }
   const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
