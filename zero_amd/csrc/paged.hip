@@ -133,15 +133,12 @@ struct Seq {
   }
 };
 
-// the last sequence that starts at or before row t of q
+// the sequence that row t of q belongs to if it belongs to one, by the ends at or before it (whole waves, one t a wave)
 __device__ __forceinline__ int seq_of(const PagedArgs& a, int t) {
-  if (t < a.B && a.cu[t] == t && a.cu[t + 1] == t + 1) return t;      // single tokens
-  int lo = 0, hi = a.B;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu[mid] <= t) lo = mid; else hi = mid;
-  }
-  return lo;
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) n += __popcll(__ballot(b0 + lane < a.B && a.cu[min(b0 + lane, a.B - 1) + 1] <= t));
+  return min(n, a.B - 1);
 }
 
 // which of the 32 keys from `base` on new token i (row q0 + i of q) may see, as bits; the cache's end is not looked at
@@ -863,33 +860,44 @@ __global__ __launch_bounds__(256) void attn_paged_merge_few_kernel(PagedArgs a) 
   else *op = f2bf(y[0] * inv);
 }
 
-// the same for the tile kernel's shares: a wave a row in turn
+// the same for the tile kernel's shares: a workgroup is a token and eight heads, a wave two of them, so that what leads to
+// the shares (four loads that wait for each other) is gone through once and the heads' loads are in flight together
 template <int HD>
 __global__ __launch_bounds__(256) void attn_paged_merge_tiles_kernel(PagedArgs a) {
-  constexpr int CPL = HD / 64;
-  const int q = a.shares[0];
+  constexpr int CPL = HD / 64, NH = 2;
+  const int q = a.shares[0], hb = (a.Hq + 7) >> 3, t = (int)blockIdx.x / hb, b = seq_of(a, t);
   if (!q) return;                                   // no sequence was shared out
   const int lane = threadIdx.x & 63, G = a.Hq / a.Hkv;
-  for (int id = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6))); id < a.T * a.Hq; id += (int)gridDim.x * 4) {
-    const int t = id / a.Hq, h = id % a.Hq, b = seq_of(a, t);
-    const Seq s(a, b);
-    const int i = t - s.q0, parts = (((s.len + 63) >> 6) + q - 1) / q;
-    if (i < 0 || i >= min(s.n, a.max_q) || parts <= 1) continue;
-    const int r = i * G + h % G;
-    const size_t p0 = (size_t)(a.shares[1 + b] + (r >> 7) * parts * a.Hkv + h / G) * 128 + (r & 127), step = (size_t)a.Hkv * 128;
-    const float* ml = a.part_ml + 2 * (p0 + lane * step);
-    const float m = lane < parts ? ml[0] : -INFINITY, l = lane < parts ? ml[1] : 0.f;
-    const float M = wave_max(m);
-    const float f = M == -INFINITY ? 0.f : fast_exp2(m - M);
-    const float L = wave_sum(l * f);
+  const int h0 = ((int)blockIdx.x % hb) * 8 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) * NH;
+  const Seq s(a, b);
+  const int i = t - s.q0, parts = (((s.len + 63) >> 6) + q - 1) / q, first = a.shares[1 + b];
+  if (i < 0 || i >= min(s.n, a.max_q) || parts <= 1) return;
+  const size_t step = (size_t)a.Hkv * 128;
+  size_t p0[NH];
+  float m[NH], l[NH];
+#pragma unroll
+  for (int x = 0; x < NH; ++x) {
+    const int h = min(h0 + x, a.Hq - 1), r = i * G + h % G;
+    p0[x] = (size_t)(first + (r >> 7) * parts * a.Hkv + h / G) * 128 + (r & 127);
+    const float* ml = a.part_ml + 2 * (p0[x] + min(lane, parts - 1) * step);
+    m[x] = ml[0];
+    l[x] = ml[1];
+  }
+#pragma unroll
+  for (int x = 0; x < NH; ++x) {
+    const float M = wave_max(m[x]);
+    const float f = M == -INFINITY || lane >= parts ? 0.f : fast_exp2(m[x] - M);
+    const float L = wave_sum(lane < parts ? l[x] * f : 0.f);
     const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
     float y[CPL];
 #pragma unroll
     for (int c = 0; c < CPL; ++c) y[c] = 0.f;
-    sum_shares<CPL>(y, a.part_o + p0 * HD + lane * CPL, step * HD, parts, f);
-    bf16_t* op = a.out + (size_t)t * a.ldo + (size_t)h * HD + lane * CPL;
-    if (CPL == 2) *reinterpret_cast<unsigned*>(op) = pack2bf(y[0] * inv, y[CPL - 1] * inv);
-    else *op = f2bf(y[0] * inv);
+    sum_shares<CPL>(y, a.part_o + p0[x] * HD + lane * CPL, step * HD, parts, f);
+    if (h0 + x < a.Hq) {
+      bf16_t* op = a.out + (size_t)t * a.ldo + (size_t)(h0 + x) * HD + lane * CPL;
+      if (CPL == 2) *reinterpret_cast<unsigned*>(op) = pack2bf(y[0] * inv, y[CPL - 1] * inv);
+      else *op = f2bf(y[0] * inv);
+    }
   }
 }
 
@@ -996,9 +1004,8 @@ extern "C" int zk_attn_paged(const void* q, const void* k_cache, const void* v_c
                       : (p.mt == 1 ? attn_paged_stream_kernel<64, 1> : p.mt == 2 ? attn_paged_stream_kernel<64, 2> : one_page ? attn_paged_tile_kernel<64, true> : attn_paged_tile_kernel<64, false>);
   hipLaunchKernelGGL(kern, dim3((unsigned)p.grid), dim3(256), 0, stream, a);
   if (p.splits > 1 && p.mt == 8) {
-    const int64_t wgs = (T * Hq + 3) / 4;
     void (*merge)(PagedArgs) = head_dim == 128 ? attn_paged_merge_tiles_kernel<128> : attn_paged_merge_tiles_kernel<64>;
-    hipLaunchKernelGGL(merge, dim3((unsigned)(wgs < 8192 ? wgs : 8192)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(merge, dim3((unsigned)(T * ((Hq + 7) / 8))), dim3(256), 0, stream, a);
   } else if (p.splits > 1) {
     // few shares: a wave a row; many of few rows: four (two) workgroups a row
     const bool few = p.splits <= 16, slices = p.splits > 64 && T * Hq < 256;
