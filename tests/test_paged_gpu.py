@@ -326,7 +326,8 @@ def differ_like(got, want, mag):
     assert ((got - want).abs()[fin] <= tol[fin]).all()
 
 
-@pytest.mark.parametrize("seqs", [[(1, 40), (3, 9)], [(8, 50), (5, 5)], [(40, 130), (70, 70)]], ids=["few", "some", "many"])
+@pytest.mark.parametrize("seqs", [[(1, 40), (3, 9)], [(8, 50), (5, 5)], [(40, 130), (70, 70)], [(1, 1100), (2, 650)],
+                                  [(40, 900), (9, 300)]], ids=["few", "some", "many", "few-shared", "many-shared"])
 @pytest.mark.parametrize("page", [16, 64])
 @pytest.mark.parametrize("tree", [False, True])
 def test_attn_paged_infinities_and_nan_reach_those_that_see_them_only(seqs, page, tree):

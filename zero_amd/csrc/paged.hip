@@ -815,7 +815,7 @@ __global__ __launch_bounds__(kMergeThreads) void attn_paged_merge_kernel(PagedAr
   a.out[(size_t)t * a.ldo + (size_t)h * HD + col0 + tid] = f2bf(v * inv);
 }
 
-// y += sum_j f[lane j] * x[j * step ..] over up to 64 shares, eight loads in flight; lanes past the last share hold f = 0
+// y += sum_j f[lane j] * x[j * step ..] over up to 64 shares, eight loads in flight
 template <int CPL>
 __device__ __forceinline__ void sum_shares(float (&y)[CPL], const float* x, size_t step, int parts, float f) {
   typedef __attribute__((ext_vector_type(CPL))) float fv;
@@ -826,8 +826,10 @@ __device__ __forceinline__ void sum_shares(float (&y)[CPL], const float* x, size
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const float w = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(f), j + u));
+      if (j + u < parts) {                          // (not by w = 0 alone: the repeated last share may be infinite)
 #pragma unroll
-      for (int c = 0; c < CPL; ++c) y[c] += v[u][c] * w;
+        for (int c = 0; c < CPL; ++c) y[c] += v[u][c] * w;
+      }
     }
   }
 }
@@ -909,7 +911,9 @@ struct Plan {
 inline Plan plan_of(int64_t B, int64_t T, int64_t max_q, int64_t max_ctx, int64_t Hq, int64_t Hkv, int64_t hd) {
   Plan p{};
   const int64_t rows = max_q * (Hq / Hkv);
-  p.mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 8;
+  // 20 rows of width 128 over 2 x 8192 (16 x 1024) keys: 23.2 (18.2) us by two 16-row groups, 24.7 (20.7) by tiles; over
+  // 8 x 4096: 39.0, 36.6.  24 rows of width 64 over 8 x 4096: 41.5 by two groups, 39.0 by tiles.  4 rows: 18 against 24.
+  p.mt = rows <= 16 ? 1 : rows <= 32 && hd == 128 ? 2 : 8;
   p.tiles = (int)((rows + 16 * p.mt - 1) / (16 * p.mt));
   const int64_t groups = B * Hkv * p.tiles;
   if (p.mt == 8) {
@@ -1001,7 +1005,7 @@ extern "C" int zk_attn_paged(const void* q, const void* k_cache, const void* v_c
   const bool one_page = page_size % 64 == 0;
   void (*kern)(PagedArgs) =
       head_dim == 128 ? (p.mt == 1 ? attn_paged_stream_kernel<128, 1> : p.mt == 2 ? attn_paged_stream_kernel<128, 2> : one_page ? attn_paged_tile_kernel<128, true> : attn_paged_tile_kernel<128, false>)
-                      : (p.mt == 1 ? attn_paged_stream_kernel<64, 1> : p.mt == 2 ? attn_paged_stream_kernel<64, 2> : one_page ? attn_paged_tile_kernel<64, true> : attn_paged_tile_kernel<64, false>);
+                      : (p.mt == 1 ? attn_paged_stream_kernel<64, 1> : one_page ? attn_paged_tile_kernel<64, true> : attn_paged_tile_kernel<64, false>);
   hipLaunchKernelGGL(kern, dim3((unsigned)p.grid), dim3(256), 0, stream, a);
   if (p.splits > 1 && p.mt == 8) {
     void (*merge)(PagedArgs) = head_dim == 128 ? attn_paged_merge_tiles_kernel<128> : attn_paged_merge_tiles_kernel<64>;
