@@ -51,7 +51,9 @@ def test_append_refusals(bad):
                                  dict(pages=0), dict(cols=0), dict(ldt=6), dict(page=1 << 20, pages=1 << 12), dict(ldq=1000),
                                  dict(ldo=1023), dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(table=None),
                                  dict(ctx=None), dict(cu=None), dict(mask=PTR, words=0), dict(q=PTR + 2), dict(k=PTR + 2),
-                                 dict(out=PTR + 8)], ids=str)
+                                 dict(out=PTR + 8), dict(scale=0.0), dict(scale=-0.1), dict(scale=float("nan")),
+                                 dict(scale=float("inf")), dict(B=1 << 30), dict(B=1 << 28, Hkv=2), dict(T=1 << 30),
+                                 dict(max_q=1 << 31), dict(max_ctx=1 << 31), dict(Hq=1 << 18, Hkv=1 << 18)], ids=str)
 def test_attention_refusals(bad):
     assert attn(**bad) == EINVAL
 
