@@ -171,7 +171,7 @@ __device__ __forceinline__ int cache_row(const PagedArgs& a, int b, int key, int
 // the XCDs in turn, so that long sequences load all of them.
 struct Work {
   int tile, split, kvh, b;
-  bool any;
+  bool any;                                         // false: an id past the last group, from rounding up to whole eights
   __device__ __forceinline__ Work(const PagedArgs& a) {
     int w = (int)(blockIdx.x >> 3);
     tile = w % a.tiles;
@@ -271,15 +271,13 @@ __device__ __forceinline__ bool not_finite(unsigned w) {
 // load); a lane then owns 8 keys of one row, which are the B operand of O^T += V^T P^T as they stand if V^T is read in
 // the same key order (elements 0-3 keys 4g.., 4-7 keys 16 + 4g.. of lane group g): ds_read_b64_tr_b16 from the wave's own
 // copy of V in LDS, chunk-swizzled by the row.  The next piece's rows are requested as soon as a piece's registers are free.
+// Bound by memory: 48 sequences of 700 to 8192 rows (8 kv heads of 128, 633 MB) 132 us, 4.8 TB/s; one of 131071 (8 heads
+// over one of 128, 67 MB) 15.7 us, 4.3 TB/s.  A short call is latency: 768 rows in 5.9 us, three dependent loads and a merge.
 // =========================================================================================
-template <int HD>
-struct Merge {
-  static constexpr int LDO = HD + 4;                // floats per row of the waves' exchange: 16 rows hit different banks
-};
-
 template <int HD, int MT>
 __global__ __launch_bounds__(256, MT == 1 && HD == 64 ? 4 : 2) void attn_paged_stream_kernel(PagedArgs a) {
-  constexpr int CPR = HD / 8, KC = HD / 32, DB = HD / 16, NV = HD / 16, LDO = Merge<HD>::LDO;
+  constexpr int CPR = HD / 8, KC = HD / 32, DB = HD / 16, NV = HD / 16;
+  constexpr int LDO = HD + 4;                       // floats per row of the waves' exchange: 16 rows hit different banks
   constexpr int VB = 32 * HD * 2;                   // one wave's V piece
   constexpr int XB = 4 * 16 * LDO * 4;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[XB > 4 * VB ? XB : 4 * VB];
@@ -518,7 +516,9 @@ __global__ __launch_bounds__(256, MT == 1 && HD == 64 ? 4 : 2) void attn_paged_s
 // the same for many rows (prompt chunks, large trees): a workgroup is 128 rows of one kv head, four waves of 32 rows that
 // share every 64-key tile.  K and V tiles arrive by LDS-DMA (per-lane 64-bit source addresses: the rows of a paged cache),
 // chunk-swizzled, two stages, one barrier per tile; S^T = K Q^T and O^T += V^T P^T in 32x32x16 MFMAs with the row on
-// the lane, as in zk_attn_fwd.  Bound by the matrix and vector pipes in turn; see that kernel's header.
+// the lane, as in zk_attn_fwd.  Each wave's instructions bind, matrix and vector in turn: a 64-key tile takes a workgroup
+// 2.5 us, of which 1.7 us stay without the matrix instructions and 2.0 us without the DMA.  2048 new tokens over 32768 rows
+// (32 heads over 8 of 128, 1.06 TFLOP): 1061 to 1129 us from card to card, 940 to 1000 TFLOP/s.  Short chunks are latency: a share's start, its stores and the merge cost as much as four of its tiles.
 // =========================================================================================
 // LDS-DMA of 16 bytes a lane to consecutive LDS from the wave-uniform `dst` on; sources per lane, or a uniform base and a
 // 32-bit byte offset.  Inline asm, not the builtin: behind a builtin the compiler waits for every DMA in flight before the
@@ -770,12 +770,13 @@ __global__ __launch_bounds__(256, kTileSlots<HD> / 256) void attn_paged_tile_ker
 }
 
 // out = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the shares of a row's sequence, in a fixed order: one workgroup
-// per (token, head, slice of COLS columns); COLS / 4 threads read a share's columns, the others every following share, and
-// the groups' sums are added in order.
+// per (token, head, slice of 32 columns); 8 threads read a share's columns, the others every following share, and the
+// groups' sums are added in order.  Slices: 512 shares of 8 rows 20.4 us a call, 24.5 with a workgroup a row; 32 of 512 rows
+// 208.4 against 206.8.
 constexpr int kMergeThreads = 256;
-template <int HD, int COLS>
+template <int HD>
 __global__ __launch_bounds__(kMergeThreads) void attn_paged_merge_kernel(PagedArgs a) {
-  constexpr int TPG = COLS / 4, NG = kMergeThreads / TPG, NSL = HD / COLS;
+  constexpr int COLS = 32, TPG = COLS / 4, NG = kMergeThreads / TPG, NSL = HD / COLS;
   __shared__ float wgt[1024];
   __shared__ __attribute__((aligned(16))) float acc[NG][COLS];
   __shared__ float red[4], sum[4];
@@ -1000,7 +1001,7 @@ extern "C" int zk_attn_paged(const void* q, const void* k_cache, const void* v_c
     return ZK_EINVAL;
   if (T == 0) return ZK_OK;
   const Plan p = plan_of(B, T, max_q, max_ctx, Hq, Hkv, head_dim);
-  if (p.grid > 0x7FFFFFF0) return ZK_EINVAL;
+  if (p.grid > 0x7FFFFFF0 || (p.mt != 8 && p.splits > 16 && T * Hq * (head_dim / 32) > 0x7FFFFFF0)) return ZK_EINVAL;
   int lg = 0;                                       // page_mul: the 31-bit reciprocal, rounded up (exact below 2^31)
   while ((int64_t)1 << lg < page_size) ++lg;
   const unsigned mul = (unsigned)((((unsigned long long)1 << (31 + lg)) / (unsigned long long)page_size) + 1);
@@ -1019,12 +1020,12 @@ extern "C" int zk_attn_paged(const void* q, const void* k_cache, const void* v_c
     void (*merge)(PagedArgs) = head_dim == 128 ? attn_paged_merge_tiles_kernel<128> : attn_paged_merge_tiles_kernel<64>;
     hipLaunchKernelGGL(merge, dim3((unsigned)(T * ((Hq + 7) / 8))), dim3(256), 0, stream, a);
   } else if (p.splits > 1) {
-    // few shares: a wave a row; many of few rows: four (two) workgroups a row
-    const bool few = p.splits <= 16, slices = p.splits > 64 && T * Hq < 256;
-    void (*merge)(PagedArgs) =
-        head_dim == 128 ? (few ? attn_paged_merge_few_kernel<128> : slices ? attn_paged_merge_kernel<128, 32> : attn_paged_merge_kernel<128, 128>)
-                        : (few ? attn_paged_merge_few_kernel<64> : slices ? attn_paged_merge_kernel<64, 32> : attn_paged_merge_kernel<64, 64>);
-    const int64_t wgs = few ? (T * Hq + 3) / 4 : T * Hq * (slices ? head_dim / 32 : 1);
+    // few shares: a wave a row (7 shares of 32 rows 8.2 us a call, 8.8 by workgroups; 4 of 1536 rows 83.7, 90.9; but 64 of
+    // 32 rows 21.1, 18.4, and 32 of 128 rows 48.2, 47.0)
+    const bool few = p.splits <= 16;
+    void (*merge)(PagedArgs) = head_dim == 128 ? (few ? attn_paged_merge_few_kernel<128> : attn_paged_merge_kernel<128>)
+                                               : (few ? attn_paged_merge_few_kernel<64> : attn_paged_merge_kernel<64>);
+    const int64_t wgs = few ? (T * Hq + 3) / 4 : T * Hq * (head_dim / 32);
     hipLaunchKernelGGL(merge, dim3((unsigned)wgs), dim3(kMergeThreads), 0, stream, a);
   }
   ZK_CHECK_LAUNCH();
