@@ -61,6 +61,44 @@ def test_sample_a_vocabulary_of_several_parts():
                [1.0, 0.9, 1.0, 0.99, 1.0, 1.0], [0.0] * 5 + [0.1])
 
 
+@pytest.mark.parametrize("V", [8192, 32768, 32769, 131072, 131073])
+def test_sample_sizes_where_the_held_row_changes(V):
+    g, rng = torch.Generator().manual_seed(V), random.Random(V)
+    x = (torch.randn(5, V, generator=g) * 3).to(BF16)
+    x[2, -1] = 30.0                                              # the last token is the only likely one
+    x[3, -9:] = torch.tensor([9.0, 8.5, 9.0, 9.5, 8.0, 9.5, 9.0, 9.5, 9.0], dtype=BF16)
+    check_rows(x, [0.3, 0.999, 0.5, 0.7, 0.0], [1.0, 0.8, 1.0, 0.3, 0.0], [0, 50, 0, 0, 0], [0.9, 1.0, 1.0, 1.0, 1.0],
+               [0.0, 0.0, 0.0, 0.02, 0.0])
+
+
+@pytest.mark.parametrize("V", [8201, 20011, 50021, 140003])
+def test_sample_largest_logits_far_behind_the_first_ones(V):
+    """The largest logit is not among the first 8192 tokens: 511, 512 and 513 values above those, or far beyond them."""
+    g, rows = torch.Generator().manual_seed(V), 12
+    x = (torch.randn(rows, V, generator=g)).to(BF16)
+    late = 8192
+    for r, key in enumerate((0x4000 + 511, 0x4000 + 512, 0x4000 + 513)):        # 0x4000: 2.0
+        x[r, :late] = x[r, :late].clamp_max(2.0)
+        x[r, 17] = 2.0
+        x[r, late + 3 + r] = torch.tensor([key], dtype=torch.int16).view(BF16)[0]
+        x[r, V - 1] = torch.tensor([key - 9], dtype=torch.int16).view(BF16)[0]
+    x[3, :late] = -math.inf                                                      # nothing but what follows
+    x[4, :late] = -1e30
+    x[5, :late] = -(2.0 ** -100)                                                 # below zero, the largest is above
+    x[5, late:] = x[5, late:] * 1e-30
+    x[6, :late] = 1e-30
+    x[7, late + 1] = math.inf
+    x[8, V - 1] = math.nan
+    x[9, :] = -math.inf
+    x[9, V - 2] = -5.0
+    x[10, :late] = x[10, :late] - 40.0
+    x[11, V - 2] = 1e20
+    T = [1.0, 30.0, 60.0, 1.0, 0.7, 1.0, 2.0, 1.0, 1.0, 1.0, 1.0, 2.0 ** 20]
+    u = [0.2, 0.99, 0.999, 0.5, 0.3, 0.6, 0.9, 0.4, 0.4, 0.4, 0.8, 0.7]
+    check_rows(x, u, T, [0, 0, 40, 0, 0, 0, 500, 0, 0, 0, 0, 0], [1.0, 1.0, 1.0, 0.9, 1.0, 1.0, 1.0, 1.0, 1.0, 1.0, 0.5, 1.0],
+               [0.0] * 8 + [0.0, 0.0, 0.05, 0.0])
+
+
 def test_sample_ties_go_to_the_lowest_index():
     x = torch.tensor([[1.0, 3.0, -0.0, 3.0, 0.0, 3.0, -0.0, 1.0]] * 8).to(BF16)
     u = [0.0, 0.3, 0.4, 0.7, 0.0, 0.999, 0.5, 0.9]

@@ -12,9 +12,10 @@
 // depend on how a sum was split: the running sum of 10^5 weights in 32 bits would move its borders by more than the
 // weight of a rare token.
 //
-// 39 936 bins (156 KiB of the CU's 160) instead of 65 281: a token further below the maximum than the last bin differs
-// from it by more than 2^28 (two bf16 of one sign are at most 32 640 values apart, so the signs differ and one of the
-// two magnitudes is beyond 2^28), and its weight is zero at every temperature up to 2^20, the largest one used.
+// 39 936 bins (156 KiB of the CU's 160) instead of 65 281: bin 0 is up to 512 values above the maximum, so a token below the
+// last bin is more than 39 423 values below the maximum.  Two bf16 of one sign are at most 32 640 values apart, so the
+// signs differ and one of the two magnitudes is beyond 2^27: weight e^-128 at 2^20, the largest temperature used, which
+// moves no sum of 2^31 weights in 64 bits.
 //
 // 128 256 tokens of one row: 23.4 us, in which one CU loads 256 KB (8 us, latency and its own bandwidth), adds to 128 256
 // LDS counts (7 us), forms the exponentials (3 us) and looks for the borders.  512 rows of 128 000 (131 MB): 60 us, two rounds
@@ -28,7 +29,7 @@ constexpr int kThreads = 1024, kWaves = kThreads / 64;
 // A thread owns 8 consecutive bins of each of 5 blocks of 8192 (occupied bins come in runs of a few thousand: a thread with
 // 39 consecutive ones would form most exponentials alone).
 constexpr int kRun = 8, kBlocks = 5, kBlock = kThreads * kRun, kBins = 39936;
-constexpr int kChunks = 16;                         // 16-byte chunks of the row a thread holds in registers
+constexpr int kChunks = 16;                         // 16-byte chunks of the row a thread holds in registers, at most
 constexpr int kRound = kThreads * 8 * kChunks;      // tokens of one register-held part of a row
 constexpr float kMaxTemperature = 1048576.0f;
 constexpr double kNothing = -64.0;                  // e^-64 of the largest weight: 2^31 such tokens do not move a 64-bit sum
@@ -50,6 +51,7 @@ struct SampleArgs {
 // tokens: every instruction per token is 0.7 us).
 typedef __attribute__((ext_vector_type(2))) short s16x2;
 constexpr int kInf = 0x7F80;
+constexpr int kAbove = 512;
 __device__ __forceinline__ unsigned keys_of(unsigned w) {
   const s16x2 m = __builtin_bit_cast(s16x2, w) >> (s16x2)15;
   return __builtin_bit_cast(unsigned, (s16x2)((__builtin_bit_cast(s16x2, w & 0x7FFF7FFFu) ^ m) - m));
@@ -58,39 +60,43 @@ __device__ __forceinline__ double value_of(int key) {
   return (double)bf2f((bf16_t)(key < 0 ? 0x8000u | (unsigned)-key : (unsigned)key));
 }
 
+typedef u32x4 u32x4_any __attribute__((aligned(2)));          // rows start at any token: 16-byte loads from 2-byte addresses
+
+// A part of a row in registers: chunk c of thread tid is tokens (c * kThreads + tid) * 8 .. of it, at p.  Chunks that the row
+// ends in or before are the last 8 tokens (so that every load is alike, and nothing waits for one early); what of them the
+// chunks before hold too becomes -inf with the keys.
+template <int NC>
 struct Row {
-  u32x4 r[kChunks];                                 // keys
-  // chunk c of the part: tokens part + (c * kThreads + tid) * 8 - skew .., where skew makes the address 16-byte aligned;
-  // `n` tokens (and skew) are left from `part` on
-  __device__ __forceinline__ void load(const bf16_t* row, long long part, int n, int skew, int tid) {
-    const bf16_t* p = row + part - skew;
-    const int lo = part ? 0 : skew;                 // valid places of the part: [lo, n)
+  u32x4 r[NC];
+  // n: tokens left from p on; at least 8 tokens up to p + n.  No branch: a wait for one chunk then leaves the later ones in
+  // flight.
+  __device__ __forceinline__ void load(const bf16_t* p, int n, int tid) {
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      u32x4 x = {0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u};     // -inf outside the row
-      if (c * kThreads * 8 < n) {
-        const int i = (c * kThreads + tid) * 8;
-        if (i >= lo && i + 8 <= n) {
-          x = *reinterpret_cast<const u32x4*>(p + i);
-        } else if (i + 8 > lo && i < n) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (i + e >= lo && i + e < n) {
-              const unsigned v = p[i + e];
-              x[e >> 1] = e & 1 ? (x[e >> 1] & 0xFFFFu) | (v << 16) : (x[e >> 1] & 0xFFFF0000u) | v;
-            }
-        }
-      }
-      r[c] = x;
-    }
+    for (int c = 0; c < NC; ++c) r[c] = *reinterpret_cast<const u32x4_any*>(p + min((c * kThreads + tid) * 8, n - 8));
   }
-  __device__ __forceinline__ void to_keys(int n) {
+  __device__ __forceinline__ void none(int c) { r[c] = u32x4{0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u}; }   // -inf
+  // the same for a row of fewer than 8 tokens, so placed that its end is the chunk's
+  __device__ __forceinline__ void load_short(const bf16_t* p, int n, int tid) {
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c)
-      if (c * kThreads * 8 < n) {
+    for (int c = 0; c < NC; ++c) none(c);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) r[c][e] = keys_of(r[c][e]);
+    for (int e = 0; e < 8; ++e)
+      if (e >= 8 - n) {
+        const unsigned v = p[e - (8 - n)];
+        r[0][e >> 1] = e & 1 ? (r[0][e >> 1] & 0xFFFFu) | (v << 16) : (r[0][e >> 1] & 0xFFFF0000u) | v;
       }
+  }
+  __device__ __forceinline__ void to_keys(int c, int n, int tid) {
+    const int s = (c * kThreads + tid) * 8 + 8 - n;
+    if (s > 0) {                                    // the first s tokens are other chunks'
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const unsigned w = r[c][e];
+        r[c][e] = s > 2 * e + 1 ? 0xFF80FF80u : s > 2 * e ? (w & 0xFFFF0000u) | 0xFF80u : w;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[c][e] = keys_of(r[c][e]);
   }
 };
 
@@ -123,22 +129,34 @@ __device__ __forceinline__ T running(const T (&v)[kBlocks], T (&before)[kBlocks]
   return lane_of(e1, kBlocks * kWaves - 64 - 1);
 }
 
-// RESIDENT: the row fits a workgroup's registers (131 072 tokens, less what its address is past 16 bytes) and is read once;
-// otherwise each pass over the row reads it again, part by part.
-template <bool RESIDENT>
+__device__ __forceinline__ void sync_lds() {       // a barrier for LDS alone: loads in flight stay in flight
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// RESIDENT: the row (8 tokens or more) fits NC chunks a thread (131 072 tokens at most) and is read once; otherwise each pass
+// over the row reads it again, part by part.
+// The counting does not wait for the row: as soon as the first 8192 tokens are there, bin 0 is put 512 values (a factor of
+// 16) above the largest of them, and every chunk is counted as it arrives (sample of 1 x 128256 23.4 -> %ONE% us, 512 rows
+// 60 -> %MANY%, against counting once the maximum is known).  If a later token is above bin 0 after all, the counts are
+// cleared and made again from the true maximum.
+template <int NC, bool RESIDENT>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   __shared__ __attribute__((aligned(16))) unsigned hist[kBins];
   __shared__ double ends_d[kBlocks * kWaves], mp_d[kWaves], cand_mass[3][kWaves], kept[3];
-  __shared__ int ends_i[kBlocks * kWaves], cand[3][kWaves], cand_count[kWaves], wtop[kWaves], wlow[kWaves], picked[2];
+  __shared__ int ends_i[kBlocks * kWaves], cand[3][kWaves], cand_count[kWaves], wtop[kWaves], wlow[kWaves], first[kWaves], picked[2];
   __shared__ __attribute__((aligned(16))) unsigned matches[kChunks * kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const long long b = blockIdx.x;
+  const long long b = blockIdx.x, V = a.V;
   const bf16_t* row = a.logits + b * a.ld;
-  const int skew = (int)((reinterpret_cast<uintptr_t>(row) & 15) >> 1);
-  const long long span = a.V + skew;
-  auto left = [&](long long part) { return RESIDENT ? (int)span : (int)min(span - part, (long long)kRound); };
-  Row x;
-  if (RESIDENT) x.load(row, 0, left(0), skew, tid);
+  auto left = [&](long long part) { return RESIDENT ? (int)V : (int)min(V - part, (long long)kRound); };
+  Row<NC> x;
+  auto read = [&](long long part) {
+    if (V >= 8) x.load(row + part, left(part), tid);
+    else x.load_short(row, (int)V, tid);
+  };
+  if (RESIDENT) x.load(row, left(0), tid);
   float Tf = a.temperature_rows ? a.temperature_rows[b] : a.temperature;
   const int top_k = a.top_k_rows ? a.top_k_rows[b] : a.top_k;
   const double top_p = a.top_p_rows ? a.top_p_rows[b] : a.top_p;
@@ -146,31 +164,59 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   const float u = a.u[b];
   const bool first_only = !(Tf > 0.f) || top_k == 1;      // the largest logit: nothing to count
   Tf = fminf(Tf, kMaxTemperature);
-  if (!first_only)
+  auto clear = [&]() {
     for (int i = tid; i < kBins / 4; i += kThreads) reinterpret_cast<u32x4*>(hist)[i] = u32x4{0u, 0u, 0u, 0u};
-  // the largest logit, and whether any is NaN
-  s16x2 hi2 = {-32768, -32768}, lo2 = {32767, 32767};
-  for (long long part = 0; part < (RESIDENT ? 1 : span); part += kRound) {
-    if (!RESIDENT) x.load(row, part, left(part), skew, tid);
-    x.to_keys(left(part));
+  };
+  int base = 0;                                     // the key of bin 0
+  // bin d counts the tokens of key base - d (a byte offset is 4 (base - key): one multiply-add; -inf has no weight)
+  auto count = [&](const u32x4& keys) {
+    const int base4 = base * 4;
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c)
+    for (int e = 0; e < 4; ++e) {
+      const unsigned w = keys[e];
+      unsigned d0, d1;
+      asm("v_mad_i32_i16 %0, %1, %2, %3" : "=v"(d0) : "v"(w), "v"(-4), "v"(base4));
+      asm("v_mad_i32_i16 %0, %1, %2, %3 op_sel:[1,0,0,0]" : "=v"(d1) : "v"(w), "v"(-4), "v"(base4));
+      if (d0 < kBins * 4u) atomicAdd(reinterpret_cast<unsigned*>(reinterpret_cast<unsigned char*>(hist) + d0), 1u);
+      if (d1 < kBins * 4u) atomicAdd(reinterpret_cast<unsigned*>(reinterpret_cast<unsigned char*>(hist) + d1), 1u);
+    }
+  };
+  if (!first_only) clear();
+  // the largest logit, whether any is NaN, and the counts
+  s16x2 hi2 = {-32768, -32768}, lo2 = {32767, 32767};
+  for (long long part = 0; part < (RESIDENT ? 1 : V); part += kRound) {
+    if (!RESIDENT) read(part);
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
       if (c * kThreads * 8 < left(part)) {
+        x.to_keys(c, left(part), tid);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const unsigned w = x.r[c][e];             // (a bit cast of a vector's element takes the vector's first one)
           hi2 = __builtin_elementwise_max(hi2, __builtin_bit_cast(s16x2, w));
           lo2 = __builtin_elementwise_min(lo2, __builtin_bit_cast(s16x2, w));
         }
+        if (!first_only) {
+          if (c == 0 && part == 0) {
+            int m = max((int)hi2[0], (int)hi2[1]);
+            m = wave_top(m);
+            if (lane == 0) first[wave] = m;
+            sync_lds();
+            m = first[lane & (kWaves - 1)];
+            m = wave_top(m);
+            base = __builtin_amdgcn_readfirstlane(min(m + kAbove, kInf));
+          }
+          count(x.r[c]);
+        }
+      } else {
+        x.none(c);
       }
   }
-  int top = max((int)hi2[0], (int)hi2[1]), low = min((int)lo2[0], (int)lo2[1]);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) { top = max(top, __shfl_xor(top, o, 64)); low = min(low, __shfl_xor(low, o, 64)); }
+  int top = wave_top(max((int)hi2[0], (int)hi2[1])), low = -wave_top(-min((int)lo2[0], (int)lo2[1]));
   if (lane == 0) { wtop[wave] = top; wlow[wave] = low; }
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) { top = max(top, wtop[w]); low = min(low, wlow[w]); }
+  top = wave_top(wtop[lane & (kWaves - 1)]);
+  low = -wave_top(-wlow[lane & (kWaves - 1)]);
   const bool nan = top > kInf || low < -kInf;
   if (nan || top == -kInf) {                        // a NaN, or no token that can be drawn
     if (tid == 0) {
@@ -182,29 +228,26 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   top = __builtin_amdgcn_readfirstlane(top);
   int bin = 0, rank = 0;
   if (!first_only) {
-    // bin d counts the tokens of key top - d (a byte offset is 4 (top - key): one multiply-add; -inf has no weight)
-    const int top4 = top * 4;
-    for (long long part = 0; part < (RESIDENT ? 1 : span); part += kRound) {
-      if (!RESIDENT) { x.load(row, part, left(part), skew, tid); x.to_keys(left(part)); }
+    if (top > base) {                               // (uniform)
+      clear();
+      base = top;
+      __syncthreads();
+      for (long long part = 0; part < (RESIDENT ? 1 : V); part += kRound) {
+        if (!RESIDENT) read(part);
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c)
-        if (c * kThreads * 8 < left(part)) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            unsigned d0, d1;
-            asm("v_mad_i32_i16 %0, %1, %2, %3" : "=v"(d0) : "v"(x.r[c][e]), "v"(-4), "v"(top4));
-            asm("v_mad_i32_i16 %0, %1, %2, %3 op_sel:[1,0,0,0]" : "=v"(d1) : "v"(x.r[c][e]), "v"(-4), "v"(top4));
-            if (d0 < kBins * 4u) atomicAdd(reinterpret_cast<unsigned*>(reinterpret_cast<unsigned char*>(hist) + d0), 1u);
-            if (d1 < kBins * 4u) atomicAdd(reinterpret_cast<unsigned*>(reinterpret_cast<unsigned char*>(hist) + d1), 1u);
+        for (int c = 0; c < NC; ++c)
+          if (c * kThreads * 8 < left(part)) {
+            if (!RESIDENT) x.to_keys(c, left(part), tid);
+            count(x.r[c]);
           }
-        }
+      }
+      __syncthreads();
     }
-    __syncthreads();
-    // weight of bin i (a maximum of +inf has the only weight)
+    // weight of bin i (a maximum of +inf has the only weight; the bins above the maximum are empty)
     const double vtop = value_of(top), inv_t = 1.0 / (double)Tf;
     auto weight = [&](int i) {
-      const double z = (value_of(top - i) - vtop) * inv_t;
-      return i == 0 ? 1.0 : z > kNothing ? exp(z) : 0.0;
+      const double z = (value_of(base - i) - vtop) * inv_t;
+      return i == base - top ? 1.0 : z > kNothing ? exp(z) : 0.0;
     };
     int cnt[kBlocks];
     double mass[kBlocks], mass_mp = 0.0;
@@ -317,7 +360,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
       }
     }
     __syncthreads();
-    bin = picked[0];
+    bin = picked[0] - (base - top);                 // from the maximum's on
     rank = picked[1];
   } else if (tid == 0) {
     a.logprobs[b] = 0.f;
@@ -325,20 +368,26 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   const int key = __builtin_amdgcn_readfirstlane(top - bin);
   const unsigned key2 = ((unsigned)key & 0xFFFFu) * 0x10001u;
   // the rank-th token (by index) of that value
-  for (long long part = 0; part < (RESIDENT ? 1 : span); part += kRound) {
-    if (!RESIDENT) { x.load(row, part, left(part), skew, tid); x.to_keys(left(part)); }
+  for (long long part = 0; part < (RESIDENT ? 1 : V); part += kRound) {
+    if (!RESIDENT) {
+      read(part);
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        if (c * kThreads * 8 < left(part)) x.to_keys(c, left(part), tid);
+        else x.none(c);
+    }
     typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
 #pragma unroll
     for (int c4 = 0; c4 < kChunks; c4 += 4) {       // most groups of chunks hold no match: one test for four
       int mine[4] = {0, 0, 0, 0};
-      if (c4 * kThreads * 8 < left(part)) {
+      if (c4 < NC && c4 * kThreads * 8 < left(part)) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           u16x2 other = {0, 0};                     // halves that differ: min(x ^ key, 1), one packed instruction in
 #pragma unroll                                      // place of the compiler's compare and select for each half
           for (int e = 0; e < 4; ++e) {
             unsigned w;
-            asm("v_pk_min_u16 %0, %1, 1 op_sel_hi:[1,0]" : "=v"(w) : "v"(x.r[c4 + k][e] ^ key2));
+            asm("v_pk_min_u16 %0, %1, 1 op_sel_hi:[1,0]" : "=v"(w) : "v"(x.r[(c4 + k) % NC][e] ^ key2));
             other += __builtin_bit_cast(u16x2, w);
           }
           const unsigned sum = __builtin_bit_cast(unsigned, other);
@@ -370,7 +419,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
       if (where % kWaves == wave) {
         u32x4 y = x.r[0];
 #pragma unroll
-        for (int c = 1; c < kChunks; ++c)
+        for (int c = 1; c < NC; ++c)
           if (c == where / kWaves) y = x.r[c];
         auto hit = [&](int e) { return ((y[e >> 1] ^ key2) & (e & 1 ? 0xFFFF0000u : 0xFFFFu)) == 0; };
         int n = 0;
@@ -381,7 +430,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
           int m = k - ex;
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (hit(e) && m-- == 0) a.tokens[b] = part + (long long)(where / kWaves * kThreads + tid) * 8 - skew + e;
+            if (hit(e) && m-- == 0) a.tokens[b] = part + min((where / kWaves * kThreads + tid) * 8, left(part) - 8) + e;
         }
       }
       return;
@@ -407,7 +456,9 @@ extern "C" int zk_sample(const void* logits, const float* u, const float* temper
   if (rows == 0) return ZK_OK;
   SampleArgs a{(const bf16_t*)logits, u, temperature_rows, top_p_rows, min_p_rows, top_k_rows, temperature, top_p, min_p,
                top_k, (long long*)tokens, logprobs, (long long)V, (long long)ld};
-  hipLaunchKernelGGL(V + 7 <= kRound ? sample_kernel<true> : sample_kernel<false>, dim3((unsigned)rows), dim3(kThreads), 0, stream, a);
+  void (*kern)(SampleArgs) = V < 8 || V > kRound ? sample_kernel<kChunks, false>
+                             : V <= kRound / 4   ? sample_kernel<kChunks / 4, true> : sample_kernel<kChunks, true>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)rows), dim3(kThreads), 0, stream, a);
   ZK_CHECK_LAUNCH();
   return ZK_OK;
 }
