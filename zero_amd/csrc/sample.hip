@@ -17,9 +17,10 @@
 // signs differ and one of the two magnitudes is beyond 2^27: weight e^-128 at 2^20, the largest temperature used, which
 // moves no sum of 2^31 weights in 64 bits.
 //
-// 128 256 tokens of one row: 23.4 us, in which one CU loads 256 KB (8 us, latency and its own bandwidth), adds to 128 256
-// LDS counts (7 us), forms the exponentials (3 us) and looks for the borders.  512 rows of 128 000 (131 MB): 60 us, two rounds
-// of 256 workgroups; 156 KiB of bins leave a CU to one row, so that the load of the next does not cover the work on this.
+// 128 256 tokens of one row: 21.1 us, 50 thousand clocks, of which the first tokens' way takes 6, the 128 256 LDS counts 20
+// (10 a wave of 64, bank conflicts of random bins), the weights 6, running sums 3, borders 4 each, the search for the token
+// 4.  512 rows of 128 256 (131 MB): 55 us, two rounds of 256 workgroups; 156 KiB of bins leave a CU to one row, so that no
+// other row's work fills these waits.  61 rows of 32 003: 15.3 us.
 #include "common.h"
 #include "../../include/zero_hip.h"
 
@@ -58,6 +59,21 @@ __device__ __forceinline__ unsigned keys_of(unsigned w) {
 }
 __device__ __forceinline__ double value_of(int key) {
   return (double)bf2f((bf16_t)(key < 0 ? 0x8000u | (unsigned)-key : (unsigned)key));
+}
+
+// e^z for z in (-64, 0]: z = n ln 2 + r with |r| <= ln 2 / 2, the Taylor series of e^r up to r^13 / 13! (what is left out is
+// 4e-18 of it), its halves side by side, and n added to the exponent.  Off by about one step of 2^-52; no special cases.
+__device__ __forceinline__ double exp_of(double z) {
+  const double n = rint(z * 1.4426950408889634);
+  double r = fma(n, -0x1.62e42fefa38p-1, z);        // ln 2 in two parts, the first with zeros behind it: n times it is exact
+  r = fma(n, -0x1.ef35793c7673p-45, r);
+  const double r2 = r * r, r4 = r2 * r2;
+  const double a = fma(fma(r, 1.0 / 6, 0.5), r2, 1.0 + r);
+  const double b = fma(fma(r, 1.0 / 5040, 1.0 / 720), r2, fma(r, 1.0 / 120, 1.0 / 24));
+  const double c = fma(fma(r, 1.0 / 39916800, 1.0 / 3628800), r2, fma(r, 1.0 / 362880, 1.0 / 40320));
+  const double d = fma(r, 1.0 / 6227020800.0, 1.0 / 479001600);
+  const double y = fma(fma(fma(d, r4, c), r4, b), r4, a);
+  return __hiloint2double(__double2hiint(y) + ((int)n << 20), __double2loint(y));
 }
 
 typedef u32x4 u32x4_any __attribute__((aligned(2)));          // rows start at any token: 16-byte loads from 2-byte addresses
@@ -138,9 +154,9 @@ __device__ __forceinline__ void sync_lds() {       // a barrier for LDS alone: l
 // RESIDENT: the row (8 tokens or more) fits NC chunks a thread (131 072 tokens at most) and is read once; otherwise each pass
 // over the row reads it again, part by part.
 // The counting does not wait for the row: as soon as the first 8192 tokens are there, bin 0 is put 512 values (a factor of
-// 16) above the largest of them, and every chunk is counted as it arrives (sample of 1 x 128256 23.4 -> %ONE% us, 512 rows
-// 60 -> %MANY%, against counting once the maximum is known).  If a later token is above bin 0 after all, the counts are
-// cleared and made again from the true maximum.
+// 16) above the largest of them, and every chunk is counted as it arrives (1 x 128256: 23.7 -> 22.0 us, 512 x 128256: 60.4 ->
+// 57.1, against counting once the maximum is known).  If a later token is above bin 0 after all, the counts are cleared and
+// made again from the true maximum.
 template <int NC, bool RESIDENT>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   __shared__ __attribute__((aligned(16))) unsigned hist[kBins];
@@ -247,7 +263,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     const double vtop = value_of(top), inv_t = 1.0 / (double)Tf;
     auto weight = [&](int i) {
       const double z = (value_of(base - i) - vtop) * inv_t;
-      return i == base - top ? 1.0 : z > kNothing ? exp(z) : 0.0;
+      return i == base - top ? 1.0 : z > kNothing ? exp_of(z) : 0.0;
     };
     int cnt[kBlocks];
     double mass[kBlocks], mass_mp = 0.0;
@@ -259,9 +275,11 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
       if (i0 >= kBins) continue;
       const u32x4 h0 = *reinterpret_cast<const u32x4*>(&hist[i0]), h1 = *reinterpret_cast<const u32x4*>(&hist[i0 + 4]);
       if (!(h0[0] | h0[1] | h0[2] | h0[3] | h1[0] | h1[1] | h1[2] | h1[3])) continue;
+      int c_next = (int)h0[0];
 #pragma unroll 1
       for (int i = i0; i < i0 + kRun; ++i) {
-        const int c = (int)hist[i];
+        const int c = c_next;
+        c_next = (int)hist[min(i + 1, kBins - 1)];
         if (!c) continue;
         const double w = weight(i), cw = (double)c * w;
         cnt[j] += c;
@@ -299,10 +317,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
       int at = 0;
       if (wave == 0) {
         const int mine = lane < kWaves ? cand[k][lane] : 0x7FFFFFFF;
-        int best = mine;
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) best = min(best, __shfl_xor(best, o, 64));
-        at = __builtin_amdgcn_readfirstlane(best);
+        at = -wave_top(-mine);
         spread(at, cand_mass[k][__ffsll(__ballot(mine == at)) - 1]);
       }
       return at;
@@ -381,21 +396,27 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     for (int c4 = 0; c4 < kChunks; c4 += 4) {       // most groups of chunks hold no match: one test for four
       int mine[4] = {0, 0, 0, 0};
       if (c4 < NC && c4 * kThreads * 8 < left(part)) {
+        u16x2 least = {0xFFFF, 0xFFFF};             // of x ^ key: zero in a half that matches
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          u16x2 other = {0, 0};                     // halves that differ: min(x ^ key, 1), one packed instruction in
-#pragma unroll                                      // place of the compiler's compare and select for each half
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
           for (int e = 0; e < 4; ++e) {
-            unsigned w;
-            asm("v_pk_min_u16 %0, %1, 1 op_sel_hi:[1,0]" : "=v"(w) : "v"(x.r[(c4 + k) % NC][e] ^ key2));
-            other += __builtin_bit_cast(u16x2, w);
+            const unsigned w = x.r[(c4 + k) % NC][e] ^ key2;
+            least = __builtin_elementwise_min(least, __builtin_bit_cast(u16x2, w));
           }
-          const unsigned sum = __builtin_bit_cast(unsigned, other);
-          mine[k] = 8 - (int)((sum & 0xFFFFu) + (sum >> 16));
-        }
-        if (__any(mine[0] | mine[1] | mine[2] | mine[3])) {
+        if (__any(least[0] == 0 || least[1] == 0)) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mine[k] = wave_upto(mine[k]);
+          for (int k = 0; k < 4; ++k) {
+            u16x2 other = {0, 0};                   // halves that differ: min(x ^ key, 1), one packed instruction in
+#pragma unroll                                      // place of the compiler's compare and select for each half
+            for (int e = 0; e < 4; ++e) {
+              unsigned w;
+              asm("v_pk_min_u16 %0, %1, 1 op_sel_hi:[1,0]" : "=v"(w) : "v"(x.r[(c4 + k) % NC][e] ^ key2));
+              other += __builtin_bit_cast(u16x2, w);
+            }
+            const unsigned sum = __builtin_bit_cast(unsigned, other);
+            mine[k] = wave_upto(8 - (int)((sum & 0xFFFFu) + (sum >> 16)));
+          }
         }
       }
       if (lane == 63) {
