@@ -122,6 +122,13 @@ def test_cache_hands_out_pages_and_takes_them_back():
             c.step(bad)
     with pytest.raises(ValueError):
         c.step([2, 0, 0], [[-1], [], []])
+    free = list(c._free)
+    for bad in ([[-1, 1], [], []], [[-1, -2], [], []], [[0, 0], [], []]):
+        with pytest.raises(ValueError, match="parent"):
+            c.step([2, 0, 0], bad)
+    with pytest.raises(ValueError):
+        c.step([-1, 2, 0])
+    assert c._free == free                                    # nothing was handed out for them
     with pytest.raises(ValueError):
         cache_of(page_size=0)
 
@@ -163,3 +170,14 @@ def test_tree_masks_and_paths():
     assert accepted_path(t, tok, [4, 7, 7, 0, 1]) == [0, 1]
     assert accepted_path(t, tok, [3, 6, 7, 0, 1]) == [0]
     assert accepted_path([-1, 0, 0], [1, 2, 2], [2, 0, 0]) == [0, 1]
+
+
+def test_generate_refuses_prompts_that_do_not_fit():
+    from types import SimpleNamespace
+    from zero_amd.inference.paged import generate_paged
+    dec = SimpleNamespace(config=SimpleNamespace(hidden_size=16), generation_config=None)
+    for prompts, more in (([], {}), ([torch.zeros(0, 16)], {}), ([torch.zeros(3, 8)], {}), ([torch.zeros(2, 3, 16)], {}),
+                          ([torch.zeros(3, 16)], dict(assistant=dec, draft_depth=0)),
+                          ([torch.zeros(3, 16)], dict(assistant=dec, assistant_prompts=[]))):
+        with pytest.raises(ValueError):
+            generate_paged(dec, prompts, 4, **more)

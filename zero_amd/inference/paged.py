@@ -124,10 +124,11 @@ class PagedKVCache:
     def step(self, counts: Sequence[int], trees: Optional[Sequence[Sequence[int]]] = None) -> Step:
         """The next ``counts[b]`` tokens of every sequence (0 allowed), behind its length, as a chain, or as the trees
         ``trees[b]`` of parents (counts[b] nodes).  The lengths move with ``advance``, so that a step may be repeated."""
-        if len(counts) != self.max_seqs or sum(counts) <= 0:
+        if len(counts) != self.max_seqs or sum(counts) <= 0 or min(counts) < 0:
             raise ValueError("step: a count for each sequence, and some token")
         if trees is not None and [len(t) for t in trees] != list(counts):
             raise ValueError("step: trees and counts differ")
+        mask = None if trees is None else tree_mask(trees, self.kv.device)       # (refuses what is no tree, before pages go)
         positions, slots, ctx, cu = [], [], [], [0]
         for b, n in enumerate(counts):
             base = self.lengths[b]
@@ -136,7 +137,6 @@ class PagedKVCache:
             slots += [self.row(b, base + i) for i in range(n)]
             ctx.append(base + n)
             cu.append(cu[-1] + n)
-        mask = None if trees is None else tree_mask(trees, self.kv.device)
         return Step(positions, slots, ctx, cu, self.page_table, mask)
 
     def advance(self, counts: Sequence[int]):
@@ -237,6 +237,10 @@ def generate_paged(decoder, prompts: Sequence[torch.Tensor], max_new_tokens: int
     with ``pad_token_id``.  ``sampling``: ops.sample's settings (None: the largest logit).  ``assistant``: a decoder of the
     same vocabulary that drafts draft_width chains of draft_depth tokens a step (its prompts default to the decoder's)."""
     tp = tp or TPContext()
+    if not prompts:
+        raise ValueError("generate: no prompts")
+    if assistant_prompts is not None and len(assistant_prompts) != len(prompts):
+        raise ValueError(f"generate: {len(assistant_prompts)} prompts for the assistant, {len(prompts)} for the decoder")
     B, device = len(prompts), prompts[0].device
     eos, pad = eos_ids(decoder, eos_token_id, pad_token_id)
     pad = 0 if pad is None else pad
@@ -254,6 +258,9 @@ def generate_paged(decoder, prompts: Sequence[torch.Tensor], max_new_tokens: int
         lens = [int(p.shape[0]) for p in rows]
         if min(lens) == 0:
             raise ValueError("generate: an empty prompt")
+        d = dec.config.hidden_size
+        if any(p.dim() != 2 or p.shape[1] != d for p in rows):
+            raise ValueError(f"generate: prompts must be [tokens, {d}] (an assistant of another width needs its own)")
         c = PagedKVCache.for_decoder(dec, B, max(lens) + max_new_tokens + nodes, device, page_size)
         st = c.step(lens)
         ends = torch.tensor([e - 1 for e in st.cu[1:]]).to(device)
