@@ -580,17 +580,17 @@ __global__ __launch_bounds__(256, kTileSlots<HD> / 256) void attn_paged_tile_ker
     else lds_dma_from(dst, src + from[ONE_PAGE ? 0 : i] + ch * 8);
   };
   row = look(0);
-  if (nt > 0) {
-    aim(row);
-#pragma unroll
-    for (int i = 0; i < 2 * NQ; ++i) piece(0, i);
-    next = look(1);
-  }
   bf16x8 qf[C::DS];
   {
     const bf16_t* qp = a.q + (size_t)(s.q0 + tok) * a.ldq + (size_t)(kvh * G + rc % G) * HD + 8 * h;
 #pragma unroll
     for (int ds = 0; ds < C::DS; ++ds) qf[ds] = *reinterpret_cast<const bf16x8*>(qp + ds * 16);
+  }
+  if (nt > 0) {
+    aim(row);
+#pragma unroll
+    for (int i = 0; i < 2 * NQ; ++i) piece(0, i);
+    next = look(1);
   }
   f32x16 o[C::DB];
 #pragma unroll
@@ -824,24 +824,30 @@ __global__ __launch_bounds__(kMergeThreads) void attn_paged_merge_kernel(PagedAr
   a.out[(size_t)t * a.ldo + (size_t)h * HD + col0 + tid] = f2bf(v * inv);
 }
 
-// y += sum_j f[lane j] * x[j * step ..] over up to 64 shares, eight loads in flight
+// y += sum_j f[lane j] * x[j * step ..] over up to 64 shares, eight loads in flight: the first eight go out with `load`, before
+// the weights f are there
 template <int CPL>
-__device__ __forceinline__ void sum_shares(float (&y)[CPL], const float* x, size_t step, int parts, float f) {
+struct ShareSum {
   typedef __attribute__((ext_vector_type(CPL))) float fv;
-  for (int j = 0; j < parts; j += 8) {
-    fv v[8];
+  fv v[8];
+  __device__ __forceinline__ void load(const float* x, size_t step, int parts, int j = 0) {
 #pragma unroll
     for (int u = 0; u < 8; ++u) v[u] = *reinterpret_cast<const fv*>(x + (size_t)min(j + u, parts - 1) * step);
+  }
+  __device__ __forceinline__ void add(float (&y)[CPL], const float* x, size_t step, int parts, float f) {
+    for (int j = 0; j < parts; j += 8) {
+      if (j) load(x, step, parts, j);
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const float w = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(f), j + u));
-      if (j + u < parts) {                          // (not by w = 0 alone: the repeated last share may be infinite)
+      for (int u = 0; u < 8; ++u) {
+        const float w = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(f), j + u));
+        if (j + u < parts) {                        // (not by w = 0 alone: the repeated last share may be infinite)
 #pragma unroll
-        for (int c = 0; c < CPL; ++c) y[c] += v[u][c] * w;
+          for (int c = 0; c < CPL; ++c) y[c] += v[u][c] * w;
+        }
       }
     }
   }
-}
+};
 
 // the same for few shares: a wave a row, HD / 64 columns a lane, four rows a workgroup
 template <int HD>
@@ -858,6 +864,8 @@ __global__ __launch_bounds__(256) void attn_paged_merge_few_kernel(PagedArgs a) 
   const float* ml = a.part_ml + (size_t)id * a.splits * 2;
   const float* po = a.part_o + (size_t)id * a.splits * HD + lane * CPL;
   float m = lane < parts ? ml[2 * lane] : -INFINITY, l = lane < parts ? ml[2 * lane + 1] : 0.f;
+  ShareSum<CPL> sum;
+  sum.load(po, HD, parts);
   const float M = wave_max(m);
   const float f = M == -INFINITY ? 0.f : fast_exp2(m - M);
   const float L = wave_sum(l * f);
@@ -865,7 +873,7 @@ __global__ __launch_bounds__(256) void attn_paged_merge_few_kernel(PagedArgs a) 
   float y[CPL];
 #pragma unroll
   for (int c = 0; c < CPL; ++c) y[c] = 0.f;
-  sum_shares<CPL>(y, po, HD, parts, f);
+  sum.add(y, po, HD, parts, f);
   bf16_t* op = a.out + (size_t)t * a.ldo + (size_t)h * HD + lane * CPL;
   if (CPL == 2) *reinterpret_cast<unsigned*>(op) = pack2bf(y[0] * inv, y[CPL - 1] * inv);
   else *op = f2bf(y[0] * inv);
@@ -894,6 +902,9 @@ __global__ __launch_bounds__(256) void attn_paged_merge_tiles_kernel(PagedArgs a
     m[x] = ml[0];
     l[x] = ml[1];
   }
+  ShareSum<CPL> sum[NH];
+#pragma unroll
+  for (int x = 0; x < NH; ++x) sum[x].load(a.part_o + p0[x] * HD + lane * CPL, step * HD, parts);
 #pragma unroll
   for (int x = 0; x < NH; ++x) {
     const float M = wave_max(m[x]);
@@ -903,7 +914,7 @@ __global__ __launch_bounds__(256) void attn_paged_merge_tiles_kernel(PagedArgs a
     float y[CPL];
 #pragma unroll
     for (int c = 0; c < CPL; ++c) y[c] = 0.f;
-    sum_shares<CPL>(y, a.part_o + p0[x] * HD + lane * CPL, step * HD, parts, f);
+    sum[x].add(y, a.part_o + p0[x] * HD + lane * CPL, step * HD, parts, f);
     if (h0 + x < a.Hq) {
       bf16_t* op = a.out + (size_t)t * a.ldo + (size_t)(h0 + x) * HD + lane * CPL;
       if (CPL == 2) *reinterpret_cast<unsigned*>(op) = pack2bf(y[0] * inv, y[CPL - 1] * inv);
