@@ -128,7 +128,7 @@ __device__ __forceinline__ T running(const T (&v)[kBlocks], T (&before)[kBlocks]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
   for (int j = 0; j < kBlocks; ++j) {
-    upto[j] = wave_upto(v[j]);
+    upto[j] = __any(v[j] != T(0)) ? wave_upto(v[j]) : T(0);     // (most waves' bins of a block are empty)
     if (lane == 63) ends[j * kWaves + wave] = upto[j];
   }
   __syncthreads();
