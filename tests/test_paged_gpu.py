@@ -306,6 +306,30 @@ def test_attn_paged_single_tokens_far_into_the_cache(ctx, Hq, Hkv, hd):
     agree(call(c), c)
 
 
+@pytest.mark.parametrize("B,ctx,Hq,Hkv,hd", [(3, 270, 4, 4, 128), (30, 700, 8, 8, 128), (6, 1023, 32, 32, 64),
+                                            (40, 300, 32, 8, 128), (70, 1000, 16, 16, 64)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_attn_paged_batches_of_short_sequences(B, ctx, Hq, Hkv, hd, tree):
+    """Lengths where eight waves take a whole sequence: up to 4 new tokens, ragged."""
+    rng = random.Random(B)
+    seqs = [(1 + b % (16 // (Hq // Hkv)) % 4, ctx) if b == 0 else (n, max(n, rng.randrange(1, ctx)))
+            for b, n in ((b, rng.choice([0, 1, 1, 2, 4])) for b in range(B))]
+    c = make(seqs, Hq, Hkv, hd, 48, tree=tree, seed=B, words=1 if tree else None)
+    agree(call(c), c)
+
+
+def test_attn_paged_whole_sequences_infinities_and_nan():
+    """The same form with infinities and NaN in new rows that only some tokens see."""
+    Hq = Hkv = 16
+    c = make([(4, 500), (2, 130), (1, 33), (3, 257), (0, 9), (4, 4), (4, 400), (2, 511)], Hq, Hkv, 64, 16, tree=True, seed=5)
+    for b, n in ((0, 4), (1, 2), (3, 3), (5, 4), (6, 4)):
+        for j, val in ((1, math.inf), (n - 1, math.nan)):
+            r = c["ctx"][b] - n + j
+            c["v"][int(c["table"][b, r // 16]), r % 16, 5 + j::17] = val
+    want, mag = ref.attention(c["q"], c["k"], c["v"], c["table"], c["ctx"], c["cu"], Hq, Hkv, 64, 0.125, c["mask"])
+    differ_like(call(c), want, torch.nan_to_num(mag, nan=0.0, posinf=0.0))
+
+
 def test_attn_paged_more_sequences_than_lanes():
     """150 sequences, some without new tokens: the layout of shares is found over several rounds of 64."""
     rng = random.Random(1)

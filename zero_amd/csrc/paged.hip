@@ -265,7 +265,7 @@ __device__ __forceinline__ bool not_finite(unsigned w) {
 // =========================================================================================
 // attention.  The q rows of a group of Hq / Hkv heads read the same keys, so a tile is 16 * MT rows (token i, head g of the
 // group at row i * G + g) of one kv head, and a workgroup is (sequence, kv head, row tile, share of the keys).
-// Four waves take 32-key pieces in turn, each with a softmax of its own (running maximum and sum in fp32, no barrier in
+// Its W waves take 32-key pieces in turn, each with a softmax of its own (running maximum and sum in fp32, no barrier in
 // the loop), merged through LDS at the end; shares of one sequence are merged by attn_paged_merge_kernel.
 // Products: 16x16x32 MFMAs.  S^T[key][row] = K Q^T, K fragments straight from memory to registers (16 rows x 64 bytes per
 // load); a lane then owns 8 keys of one row, which are the B operand of O^T += V^T P^T as they stand if V^T is read in
@@ -274,14 +274,14 @@ __device__ __forceinline__ bool not_finite(unsigned w) {
 // Bound by memory: 48 sequences of 700 to 8192 rows (8 kv heads of 128, 633 MB) 132 us, 4.8 TB/s; one of 131071 (8 heads
 // over one of 128, 67 MB) 15.7 us, 4.3 TB/s.  A short call is latency: 768 rows in 5.9 us, three dependent loads and a merge.
 // =========================================================================================
-template <int HD, int MT>
-__global__ __launch_bounds__(256, MT == 1 && HD == 64 ? 4 : 2) void attn_paged_stream_kernel(PagedArgs a) {
+template <int HD, int MT, int W>
+__global__ __launch_bounds__(64 * W, W == 4 && MT == 1 && HD == 64 ? 4 : 2) void attn_paged_stream_kernel(PagedArgs a) {
   constexpr int CPR = HD / 8, KC = HD / 32, DB = HD / 16, NV = HD / 16;
   constexpr int LDO = HD + 4;                       // floats per row of the waves' exchange: 16 rows hit different banks
   constexpr int VB = 32 * HD * 2;                   // one wave's V piece
-  constexpr int XB = 4 * 16 * LDO * 4;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[XB > 4 * VB ? XB : 4 * VB];
-  __shared__ float sm[4][16 * MT], sl[4][16 * MT];
+  constexpr int XB = W * 16 * LDO * 4;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[XB > W * VB ? XB : W * VB];
+  __shared__ float sm[W][16 * MT], sl[W][16 * MT];
   const int tid = threadIdx.x, lane = tid & 63, g4 = lane >> 4, col = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Work w(a);
@@ -393,17 +393,17 @@ __global__ __launch_bounds__(256, MT == 1 && HD == 64 ? 4 : 2) void attn_paged_s
   if (base + 32 <= bulk) {
     int row = cache_row(a, b, base + (lane & 31), bulk);
     request(row);
-    int ahead = cache_row(a, b, base + 128 + (lane & 31), bulk);
+    int ahead = cache_row(a, b, base + 32 * W + (lane & 31), bulk);
     while (__all(row >= 0)) {
       scores();
 #pragma unroll
       for (int i = 0; i < NV; ++i) *reinterpret_cast<u32x4*>(v_at((i * 64 + lane) / CPR, (i * 64 + lane) % CPR)) = vr[i];
       lds_turn();
-      base += 128;
+      base += 32 * W;
       row = ahead;
       if (base + 32 <= bulk) {
         request(row);
-        ahead = cache_row(a, b, base + 128 + (lane & 31), bulk);
+        ahead = cache_row(a, b, base + 32 * W + (lane & 31), bulk);
       }
       softmax();
       product();
@@ -412,7 +412,7 @@ __global__ __launch_bounds__(256, MT == 1 && HD == 64 ? 4 : 2) void attn_paged_s
     }
   }
   // the others: the cache's end, new tokens, pages that do not exist (and what stands behind one)
-  for (; base < ke; base += 128) {
+  for (; base < ke; base += 32 * W) {
     const int row = cache_row(a, b, base + (lane & 31), ke);
     request(row);
     scores();
@@ -461,7 +461,7 @@ __global__ __launch_bounds__(256, MT == 1 && HD == 64 ? 4 : 2) void attn_paged_s
     }
     lds_turn();
   }
-  // ---- the four waves' shares, in wave order
+  // ---- the waves' shares, in wave order
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     l[mt] += __shfl_xor(l[mt], 16, 64);
@@ -469,13 +469,20 @@ __global__ __launch_bounds__(256, MT == 1 && HD == 64 ? 4 : 2) void attn_paged_s
     if (g4 == 0) { sm[wave][mt * 16 + col] = m[mt]; sl[wave][mt * 16 + col] = l[mt]; }
   }
   float* xo = reinterpret_cast<float*>(smem);
-  const int per = HD / 16, orow = tid >> 4, oc = (tid & 15) * per;
+  constexpr int per = HD / (4 * W);                  // columns a thread writes
+  const int orow = tid / (4 * W), oc = (tid % (4 * W)) * per;
+  auto top = [&](int r) {
+    float M = sm[0][r];
+#pragma unroll
+    for (int w = 1; w < W; ++w) M = fmaxf(M, sm[w][r]);
+    return M;
+  };
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     __syncthreads();
     {
       const int r = mt * 16 + col;
-      const float M = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
+      const float M = top(r);
       const float f = M == -INFINITY ? 0.f : fast_exp2(m[mt] - M);
 #pragma unroll
       for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4*>(xo + (wave * 16 + col) * LDO + d * 16 + 4 * g4) = o[mt][d] * f;
@@ -484,28 +491,36 @@ __global__ __launch_bounds__(256, MT == 1 && HD == 64 ? 4 : 2) void attn_paged_s
     const int r = r0 + mt * 16 + orow;
     if (r < rows) {
       const int lr = mt * 16 + orow;
-      const float M = fmaxf(fmaxf(sm[0][lr], sm[1][lr]), fmaxf(sm[2][lr], sm[3][lr]));
+      const float M = top(lr);
       float L = 0.f, y[per];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) L += M == -INFINITY ? 0.f : sl[w][lr] * fast_exp2(sm[w][lr] - M);
+      for (int w = 0; w < W; ++w) L += M == -INFINITY ? 0.f : sl[w][lr] * fast_exp2(sm[w][lr] - M);
 #pragma unroll
-      for (int e = 0; e < per; ++e)
-        y[e] = (xo[orow * LDO + oc + e] + xo[(16 + orow) * LDO + oc + e]) +
-               (xo[(32 + orow) * LDO + oc + e] + xo[(48 + orow) * LDO + oc + e]);
+      for (int e = 0; e < per; ++e) {
+        y[e] = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; w += 4)
+          y[e] += (xo[(16 * w + orow) * LDO + oc + e] + xo[(16 * w + 16 + orow) * LDO + oc + e]) +
+                  (xo[(16 * w + 32 + orow) * LDO + oc + e] + xo[(16 * w + 48 + orow) * LDO + oc + e]);
+      }
       const int t = s.q0 + r / G, h = kvh * G + r % G;
       if (alone) {
         const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);      // nothing seen: zeros; NaN stays NaN
         bf16_t* op = a.out + (size_t)t * a.ldo + (size_t)h * HD + oc;
 #pragma unroll
-        for (int e = 0; e < per; e += 4) {
-          u32x2 w = {pack2bf(y[e] * inv, y[e + 1] * inv), pack2bf(y[e + 2] * inv, y[e + 3] * inv)};
-          *reinterpret_cast<u32x2*>(op + e) = w;
-        }
+        for (int e = 0; e < per; e += W == 4 ? 4 : 2)
+          if constexpr (W == 4) {
+            u32x2 w = {pack2bf(y[e] * inv, y[e + 1] * inv), pack2bf(y[e + 2] * inv, y[e + 3] * inv)};
+            *reinterpret_cast<u32x2*>(op + e) = w;
+          } else {
+            *reinterpret_cast<unsigned*>(op + e) = pack2bf(y[e] * inv, y[e + 1] * inv);
+          }
       } else {
         const size_t part = ((size_t)t * a.Hq + h) * a.splits + split;
 #pragma unroll
-        for (int e = 0; e < per; e += 4)
-          *reinterpret_cast<f32x4*>(a.part_o + part * HD + oc + e) = f32x4{y[e], y[e + 1], y[e + 2], y[e + 3]};
+        for (int e = 0; e < per; e += 4)            // (8 waves: no call has shares)
+          if constexpr (W == 4)
+            *reinterpret_cast<f32x4*>(a.part_o + part * HD + oc + e) = f32x4{y[e], y[e + 1], y[e + 2], y[e + 3]};
         if (oc == 0) { a.part_ml[part * 2] = M; a.part_ml[part * 2 + 1] = L; }
       }
     }
@@ -926,7 +941,7 @@ __global__ __launch_bounds__(256) void attn_paged_merge_tiles_kernel(PagedArgs a
 
 // shape of a launch: host arithmetic on the sizes alone
 struct Plan {
-  int mt, tiles, splits, split_keys;                // mt: 16-row groups of the stream kernel's tile, 8 = the tile kernel
+  int mt, waves, tiles, splits, split_keys;         // mt: 16-row groups of the stream kernel's tile, 8 = the tile kernel
   int64_t grid, header, parts, ws;                  // workgroups; floats of the header, parts, floats altogether
 };
 inline Plan plan_of(int64_t B, int64_t T, int64_t max_q, int64_t max_ctx, int64_t Hq, int64_t Hkv, int64_t hd) {
@@ -952,6 +967,16 @@ inline Plan plan_of(int64_t B, int64_t T, int64_t max_q, int64_t max_ctx, int64_
     int64_t keys = (max_ctx * groups + 511) / 512;
     keys = (keys + 127) / 128 * 128;
     keys = keys < 128 ? 128 : keys > 512 ? 512 : keys;
+    p.waves = 4;
+    // No shares and no merge, but eight waves, where that costs less than a merge (3 us): what the CUs without a workgroup
+    // would have taken off the longest sequence's K and V, at the 46 GB/s that a CU reads, is 140 KB; and not above 512 KB,
+    // as lengths differ.  (32 over 8 of 128: 24 x 512 keys 12.7 us, 16.0 by shares; 24 x 1024 21.0, 25.4; 64 x 771 35.9,
+    // 39.7; 8 x 256 6.8, 7.8; but 8 x 512 9.6, 7.8.  16 of 64: 8 x 512 6.6, 8.2; 1 x 512 6.1, 7.0; 1 x 771 8.2, 7.2)
+    const int64_t bytes = max_ctx * hd * 4, idle = groups < 256 ? 256 - groups : 0;
+    if (p.mt == 1 && keys < max_ctx && bytes <= (512 << 10) && bytes * idle <= 256 * (140 << 10)) {
+      keys = max_ctx;
+      p.waves = 8;
+    }
     p.split_keys = (int)keys;
     p.splits = (int)((max_ctx + keys - 1) / keys);
     p.grid = (B * Hkv * p.splits + 7) / 8 * 8 * p.tiles;
@@ -1025,9 +1050,9 @@ extern "C" int zk_attn_paged(const void* q, const void* k_cache, const void* v_c
               (long long)ldq, (long long)ldo, scale};
   const bool one_page = page_size % 64 == 0;
   void (*kern)(PagedArgs) =
-      head_dim == 128 ? (p.mt == 1 ? attn_paged_stream_kernel<128, 1> : p.mt == 2 ? attn_paged_stream_kernel<128, 2> : one_page ? attn_paged_tile_kernel<128, true> : attn_paged_tile_kernel<128, false>)
-                      : (p.mt == 1 ? attn_paged_stream_kernel<64, 1> : one_page ? attn_paged_tile_kernel<64, true> : attn_paged_tile_kernel<64, false>);
-  hipLaunchKernelGGL(kern, dim3((unsigned)p.grid), dim3(256), 0, stream, a);
+      head_dim == 128 ? (p.mt == 1 ? (p.waves == 4 ? attn_paged_stream_kernel<128, 1, 4> : attn_paged_stream_kernel<128, 1, 8>) : p.mt == 2 ? attn_paged_stream_kernel<128, 2, 4> : one_page ? attn_paged_tile_kernel<128, true> : attn_paged_tile_kernel<128, false>)
+                      : (p.mt == 1 ? (p.waves == 4 ? attn_paged_stream_kernel<64, 1, 4> : attn_paged_stream_kernel<64, 1, 8>) : one_page ? attn_paged_tile_kernel<64, true> : attn_paged_tile_kernel<64, false>);
+  hipLaunchKernelGGL(kern, dim3((unsigned)p.grid), dim3(p.waves == 8 ? 512 : 256), 0, stream, a);
   if (p.splits > 1 && p.mt == 8) {
     void (*merge)(PagedArgs) = head_dim == 128 ? attn_paged_merge_tiles_kernel<128> : attn_paged_merge_tiles_kernel<64>;
     hipLaunchKernelGGL(merge, dim3((unsigned)(T * ((Hq + 7) / 8))), dim3(256), 0, stream, a);
