@@ -299,6 +299,13 @@ def test_attn_paged_shares_of_long_ragged_sequences(Hq, Hkv, hd, page, tree):
     agree(call(c), c)
 
 
+@pytest.mark.parametrize("Hq,Hkv,hd,tree", [(20, 2, 64, False), (17, 1, 128, False), (20, 4, 128, True)])
+def test_attn_paged_shares_of_many_rows(Hq, Hkv, hd, tree):
+    """More rows than waves fit the GPU at once, some of their sequences shared out; heads that no group of eight ends with."""
+    c = make([(300, 1900), (250, 700), (1, 900)], Hq, Hkv, hd, 32, tree=tree, seed=24)
+    agree(call(c), c)
+
+
 @pytest.mark.parametrize("ctx", [5000, 40001])
 @pytest.mark.parametrize("Hq,Hkv,hd", [(8, 1, 128), (4, 2, 64), (40, 2, 128)])
 def test_attn_paged_single_tokens_far_into_the_cache(ctx, Hq, Hkv, hd):

@@ -895,15 +895,15 @@ __global__ __launch_bounds__(256) void attn_paged_merge_few_kernel(PagedArgs a) 
   else *op = f2bf(y[0] * inv);
 }
 
-// the same for the tile kernel's shares: a workgroup is a token and eight heads, a wave two of them, so that what leads to
-// the shares (four loads that wait for each other) is gone through once and the heads' loads are in flight together
-template <int HD>
+// the same for the tile kernel's shares: a workgroup is a token and 4 NH heads, a wave NH of them, so that what leads to the
+// shares (four loads that wait for each other) is gone through once and the heads' loads are in flight together
+template <int HD, int NH>
 __global__ __launch_bounds__(256) void attn_paged_merge_tiles_kernel(PagedArgs a) {
-  constexpr int CPL = HD / 64, NH = 2;
-  const int q = a.shares[0], hb = (a.Hq + 7) >> 3, t = (int)blockIdx.x / hb, b = seq_of(a, t);
+  constexpr int CPL = HD / 64;
+  const int q = a.shares[0], hb = (a.Hq + 4 * NH - 1) / (4 * NH), t = (int)blockIdx.x / hb, b = seq_of(a, t);
   if (!q) return;                                   // no sequence was shared out
   const int lane = threadIdx.x & 63, G = a.Hq / a.Hkv;
-  const int h0 = ((int)blockIdx.x % hb) * 8 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) * NH;
+  const int h0 = ((int)blockIdx.x % hb) * 4 * NH + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) * NH;
   const Seq s(a, b);
   const int i = t - s.q0, parts = (((s.len + 63) >> 6) + q - 1) / q, first = a.shares[1 + b];
   if (i < 0 || i >= min(s.n, a.max_q) || parts <= 1) return;
@@ -1054,8 +1054,13 @@ extern "C" int zk_attn_paged(const void* q, const void* k_cache, const void* v_c
                       : (p.mt == 1 ? (p.waves == 4 ? attn_paged_stream_kernel<64, 1, 4> : attn_paged_stream_kernel<64, 1, 8>) : one_page ? attn_paged_tile_kernel<64, true> : attn_paged_tile_kernel<64, false>);
   hipLaunchKernelGGL(kern, dim3((unsigned)p.grid), dim3(p.waves == 8 ? 512 : 256), 0, stream, a);
   if (p.splits > 1 && p.mt == 8) {
-    void (*merge)(PagedArgs) = head_dim == 128 ? attn_paged_merge_tiles_kernel<128> : attn_paged_merge_tiles_kernel<64>;
-    hipLaunchKernelGGL(merge, dim3((unsigned)(T * ((Hq + 7) / 8))), dim3(256), 0, stream, a);
+    // a wave a row while every row's wave is resident at once (256 CUs x 32): 160 rows x 8 heads of 50 shares 33.2 -> 31.4 us
+    // a call, 89 x 2 x 8 31.3 -> 28.6; beyond, two rows a wave: 1000 x 16 48.6, 51.3 by one
+    const bool one = T * Hq <= 8192;
+    void (*merge)(PagedArgs) = head_dim == 128 ? (one ? attn_paged_merge_tiles_kernel<128, 1> : attn_paged_merge_tiles_kernel<128, 2>)
+                                               : (one ? attn_paged_merge_tiles_kernel<64, 1> : attn_paged_merge_tiles_kernel<64, 2>);
+    const int64_t heads = one ? 4 : 8;
+    hipLaunchKernelGGL(merge, dim3((unsigned)(T * ((Hq + heads - 1) / heads))), dim3(256), 0, stream, a);
   } else if (p.splits > 1) {
     // few shares: a wave a row (7 shares of 32 rows 8.2 us a call, 8.8 by workgroups; 4 of 1536 rows 83.7, 90.9; but 64 of
     // 32 rows 21.1, 18.4, and 32 of 128 rows 48.2, 47.0)
