@@ -99,6 +99,34 @@ def test_sample_largest_logits_far_behind_the_first_ones(V):
                [0.0] * 8 + [0.0, 0.0, 0.05, 0.0])
 
 
+@pytest.mark.parametrize("V", [8, 300, 4681, 32768])
+def test_sample_many_rows_as_few(V):
+    """More rows than CUs are counted in 16 bits, two rows a CU: the same tokens as in small batches, and the sorted rows'."""
+    from zero_amd import ops
+    g, rng, rows = torch.Generator().manual_seed(V), random.Random(V), 300
+    x = (torch.randn(rows, V, generator=g) * 3).to(BF16)
+    x[5] = 1.5                                                   # one value: a count of V
+    x[6, ::2], x[6, 1::2] = 2.0, torch.tensor([0x4001], dtype=torch.int16).view(BF16)[0]    # two neighbouring values
+    x[7] = -math.inf
+    x[8, V - 1] = math.nan
+    x[9, : V // 2] = -math.inf
+    u = torch.tensor([rng.random() * (1 - 2.0 ** -23) for _ in range(rows)])
+    T, k, p, mp = settings(rng, rows)
+    T[5], k[5], p[5], mp[5], T[6], k[6], p[6], mp[6] = 1.0, 0, 1.0, 0.0, 1.0, 0, 1.0, 0.0
+    par = [torch.tensor(T, device=DEV), torch.tensor(k, dtype=torch.int32, device=DEV), torch.tensor(p, device=DEV),
+           torch.tensor(mp, device=DEV)]
+    xd, ud = x.to(DEV), u.to(DEV)
+    tok, logp = ops.sample(xd, ud, *par)
+    halves = [ops.sample(xd[s], ud[s], *[v[s] for v in par]) for s in (slice(0, 150), slice(150, rows))]
+    assert torch.equal(tok, torch.cat([h[0] for h in halves]))
+    assert torch.equal(logp.nan_to_num(7.0), torch.cat([h[1] for h in halves]).nan_to_num(7.0))
+    for r in list(range(4, 11)) + [200, 299]:
+        t, lp = ref.sample_row(x[r].double().tolist(), float(u[r]), f32(T[r]), k[r], f32(p[r]), f32(mp[r]))
+        got = float(logp[r])
+        assert int(tok[r]) == t, (r, int(tok[r]), t)
+        assert got == lp or (math.isnan(got) and math.isnan(lp)) or abs(got - lp) <= 2.0 ** -24 * abs(lp) + 1e-12, (r, got, lp)
+
+
 def test_sample_ties_go_to_the_lowest_index():
     x = torch.tensor([[1.0, 3.0, -0.0, 3.0, 0.0, 3.0, -0.0, 1.0]] * 8).to(BF16)
     u = [0.0, 0.3, 0.4, 0.7, 0.0, 0.999, 0.5, 0.9]

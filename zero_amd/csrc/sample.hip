@@ -153,16 +153,18 @@ __device__ __forceinline__ void sync_lds() {       // a barrier for LDS alone: l
 
 // RESIDENT: the row (8 tokens or more) fits NC chunks a thread (131 072 tokens at most) and is read once; otherwise each pass
 // over the row reads it again, part by part.
+// HALF: the bins are 16 bits wide (rows of up to 32 768 tokens).
 // The counting does not wait for the row: as soon as the first 8192 tokens are there, bin 0 is put 512 values (a factor of
 // 16) above the largest of them, and every chunk is counted as it arrives (1 x 128256: 23.7 -> 22.0 us, 512 x 128256: 60.4 ->
 // 57.1, against counting once the maximum is known).  If a later token is above bin 0 after all, the counts are cleared and
 // made again from the true maximum.
-template <int NC, bool RESIDENT>
-__global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
-  __shared__ __attribute__((aligned(16))) unsigned hist[kBins];
+template <int NC, bool RESIDENT, bool HALF>
+__global__ __launch_bounds__(kThreads, HALF ? 8 : 4) void sample_kernel(SampleArgs a) {
+  __shared__ __attribute__((aligned(16))) unsigned hist[HALF ? kBins / 2 : kBins];
+  auto counted = [&](int i) { return HALF ? (int)reinterpret_cast<const unsigned short*>(hist)[i] : (int)hist[i]; };
   __shared__ double ends_d[kBlocks * kWaves], mp_d[kWaves], cand_mass[3][kWaves], kept[3];
   __shared__ int ends_i[kBlocks * kWaves], cand[3][kWaves], cand_count[kWaves], wtop[kWaves], wlow[kWaves], first[kWaves], picked[2];
-  __shared__ __attribute__((aligned(16))) unsigned matches[kChunks * kWaves];
+  unsigned* matches = hist;                         // [kChunks * kWaves], once the counts are done with
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const long long b = blockIdx.x, V = a.V;
   const bf16_t* row = a.logits + b * a.ld;
@@ -181,20 +183,29 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   const bool first_only = !(Tf > 0.f) || top_k == 1;      // the largest logit: nothing to count
   Tf = fminf(Tf, kMaxTemperature);
   auto clear = [&]() {
-    for (int i = tid; i < kBins / 4; i += kThreads) reinterpret_cast<u32x4*>(hist)[i] = u32x4{0u, 0u, 0u, 0u};
+    for (int i = tid; i < kBins / (HALF ? 8 : 4); i += kThreads) reinterpret_cast<u32x4*>(hist)[i] = u32x4{0u, 0u, 0u, 0u};
   };
   int base = 0;                                     // the key of bin 0
-  // bin d counts the tokens of key base - d (a byte offset is 4 (base - key): one multiply-add; -inf has no weight)
+  // bin d counts the tokens of key base - d (its byte offset is one multiply-add; -inf has no weight)
+  constexpr int BB = HALF ? 2 : 4;                  // bytes a bin
   auto count = [&](const u32x4& keys) {
-    const int base4 = base * 4;
+    const int base_b = base * BB, base16 = base * 16;
+    auto add = [&](unsigned d, unsigned d16) __attribute__((always_inline)) {
+      if (d < (unsigned)kBins * BB)                 // (half: 16 d is 0 or 16 in the five bits of a shift)
+        atomicAdd(reinterpret_cast<unsigned*>(reinterpret_cast<unsigned char*>(hist) + (HALF ? d & ~3u : d)), HALF ? 1u << (d16 & 31) : 1u);
+    };
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const unsigned w = keys[e];
-      unsigned d0, d1;
-      asm("v_mad_i32_i16 %0, %1, %2, %3" : "=v"(d0) : "v"(w), "v"(-4), "v"(base4));
-      asm("v_mad_i32_i16 %0, %1, %2, %3 op_sel:[1,0,0,0]" : "=v"(d1) : "v"(w), "v"(-4), "v"(base4));
-      if (d0 < kBins * 4u) atomicAdd(reinterpret_cast<unsigned*>(reinterpret_cast<unsigned char*>(hist) + d0), 1u);
-      if (d1 < kBins * 4u) atomicAdd(reinterpret_cast<unsigned*>(reinterpret_cast<unsigned char*>(hist) + d1), 1u);
+      unsigned d0, d1, s0 = 0, s1 = 0;
+      asm("v_mad_i32_i16 %0, %1, %2, %3" : "=v"(d0) : "v"(w), "v"(-BB), "v"(base_b));
+      asm("v_mad_i32_i16 %0, %1, %2, %3 op_sel:[1,0,0,0]" : "=v"(d1) : "v"(w), "v"(-BB), "v"(base_b));
+      if (HALF) {
+        asm("v_mad_i32_i16 %0, %1, %2, %3" : "=v"(s0) : "v"(w), "v"(-16), "v"(base16));
+        asm("v_mad_i32_i16 %0, %1, %2, %3 op_sel:[1,0,0,0]" : "=v"(s1) : "v"(w), "v"(-16), "v"(base16));
+      }
+      add(d0, s0);
+      add(d1, s1);
     }
   };
   if (!first_only) clear();
@@ -273,13 +284,14 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
       mass[j] = 0.0;
       const int i0 = j * kBlock + tid * kRun;
       if (i0 >= kBins) continue;
-      const u32x4 h0 = *reinterpret_cast<const u32x4*>(&hist[i0]), h1 = *reinterpret_cast<const u32x4*>(&hist[i0 + 4]);
-      if (!(h0[0] | h0[1] | h0[2] | h0[3] | h1[0] | h1[1] | h1[2] | h1[3])) continue;
-      int c_next = (int)h0[0];
+      u32x4 any = *reinterpret_cast<const u32x4*>(&hist[HALF ? i0 / 2 : i0]);
+      if (!HALF) any |= *reinterpret_cast<const u32x4*>(&hist[i0 + 4]);
+      if (!(any[0] | any[1] | any[2] | any[3])) continue;
+      int c_next = counted(i0);
 #pragma unroll 1
       for (int i = i0; i < i0 + kRun; ++i) {
         const int c = c_next;
-        c_next = (int)hist[min(i + 1, kBins - 1)];
+        c_next = counted(min(i + 1, kBins - 1));
         if (!c) continue;
         const double w = weight(i), cw = (double)c * w;
         cnt[j] += c;
@@ -298,7 +310,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     double w8 = 0.0, run8 = 0.0;
     auto spread = [&](int at, double from) {
       const int i = at * kRun + (lane & 7);         // thread t of block j: at = j * kThreads + t
-      c8 = (int)hist[i];
+      c8 = counted(i);
       w8 = c8 ? weight(i) : 0.0;
       double v = (double)c8 * w8;
       v += dpp0<0x111, 0xF>(v) * (double)((lane & 7) >= 1);
@@ -477,8 +489,13 @@ extern "C" int zk_sample(const void* logits, const float* u, const float* temper
   if (rows == 0) return ZK_OK;
   SampleArgs a{(const bf16_t*)logits, u, temperature_rows, top_p_rows, min_p_rows, top_k_rows, temperature, top_p, min_p,
                top_k, (long long*)tokens, logprobs, (long long)V, (long long)ld};
-  void (*kern)(SampleArgs) = V < 8 || V > kRound ? sample_kernel<kChunks, false>
-                             : V <= kRound / 4   ? sample_kernel<kChunks / 4, true> : sample_kernel<kChunks, true>;
+  // more rows than CUs, and few enough tokens for counts of 16 bits: 78 KiB of bins, so that two rows share a CU and one works
+  // while the other waits (1024 x 300 43 -> 31 us, 512 x 4681 23.9 -> 19.6, 512 x 32003 28.7 -> 26.3; but 256 x 32003 15.0 ->
+  // 17.7, on half the registers and with more instructions a count)
+  const bool two = rows > 256;
+  void (*kern)(SampleArgs) = V < 8 || V > kRound ? sample_kernel<kChunks, false, false>
+                             : V > kRound / 4    ? sample_kernel<kChunks, true, false>
+                             : two               ? sample_kernel<kChunks / 4, true, true> : sample_kernel<kChunks / 4, true, false>;
   hipLaunchKernelGGL(kern, dim3((unsigned)rows), dim3(kThreads), 0, stream, a);
   ZK_CHECK_LAUNCH();
   return ZK_OK;
