@@ -5,9 +5,9 @@
 //   tokens with w >= min_p.  All three are prefixes of one order, so the kept set is the shortest of them, and the token
 //   drawn is the first whose running sum exceeds u * Z, Z = the kept sum.  logprob = log(w / Z).
 //
-// bf16 logits have at most 65 281 different values that can be drawn, so the sorted row is its HISTOGRAM: bin d (0 = the
-// largest value's bin) holds how many tokens have that value, a bin of c tokens adds c * w(d) to the running sum, and no
-// sort of 10^5 tokens is needed.  One workgroup owns a row; its bins live in LDS as 32-bit counts.  Sums are formed in
+// bf16 logits have at most 65 281 different values that can be drawn, so the sorted row is its HISTOGRAM: bins in
+// falling order of the value hold how many tokens have it, a bin of c tokens adds c * w to the running sum, and no sort
+// of 10^5 tokens is needed.  One workgroup owns a row; its bins live in LDS as 32-bit counts (see HALF).  Sums are formed in
 // 64 bits over the occupied bins only (a few thousand exponentials instead of one per token), so that the token does not
 // depend on how a sum was split: the running sum of 10^5 weights in 32 bits would move its borders by more than the
 // weight of a rare token.
