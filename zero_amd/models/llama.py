@@ -68,24 +68,27 @@ TAIL_ROWS_USED = 0          # forwards that took the row-restricted tail (tests)
 
 class LlamaRotaryEmbedding(nn.Module):
     """cos/sin tables [S, head_dim/2] in fp32 holding the bf16-rounded values (tf:llama:113-127:
-    fp32 outer product, cos/sin, cast to the activation dtype).  Built on the host once per
-    sequence length and cached on the device."""
+    fp32 outer product, cos/sin, cast to the activation dtype).  Built on the host; what is handed out are the first S
+    rows of one device table, which is made anew, at least twice as long, when it is too short.  The shorter ones stay as
+    long as the module (together they are no longer than the last): captured graphs and native plans read them by address."""
 
     def __init__(self, cfg: LlamaConfig):
         super().__init__()
         self.cfg = cfg
-        self._cache: Dict = {}
+        self._cache: Dict = {}                             # device -> [(cos, sin), ...], the longest last
 
     def tables(self, S: int, device):
-        key = (S, str(device))
-        if key not in self._cache:
-            inv = llama3_inv_freq(self.cfg)
-            pos = torch.arange(S, dtype=torch.float32)
-            freqs = (inv[:, None] @ pos[None, :]).transpose(0, 1)          # [S, hd/2]
-            cos = freqs.cos().to(torch.bfloat16).to(torch.float32)
-            sin = freqs.sin().to(torch.bfloat16).to(torch.float32)
-            self._cache = {key: (cos.contiguous().to(device), sin.contiguous().to(device))}
-        return self._cache[key]
+        made = self._cache.setdefault(str(device), [])
+        if not made or made[-1][0].shape[0] < S:
+            with torch.inference_mode(False), torch.no_grad():             # (a later training step saves views of them)
+                inv = llama3_inv_freq(self.cfg)
+                pos = torch.arange(1 << max(S - 1, 1023).bit_length(), dtype=torch.float32)
+                freqs = (inv[:, None] @ pos[None, :]).transpose(0, 1)      # [rows, hd/2]
+                cos = freqs.cos().to(torch.bfloat16).to(torch.float32)
+                sin = freqs.sin().to(torch.bfloat16).to(torch.float32)
+                made.append((cos.contiguous().to(device), sin.contiguous().to(device)))
+        cos, sin = made[-1]
+        return cos[:S], sin[:S]
 
 
 class LlamaAttention(nn.Module):
