@@ -1,5 +1,6 @@
 """The rotary tables' lifetime and values: kernels, captured graphs and DecodePlan read them by address."""
 import gc
+import weakref
 
 import pytest
 import torch
@@ -65,3 +66,17 @@ def test_tables_made_in_inference_mode_serve_training():
     x = torch.ones(33, 32, requires_grad=True)
     (x * cos).sum().backward()                               # (cos is saved for the gradient)
     assert torch.equal(x.grad, cos)
+
+
+def test_decode_plan_holds_the_tables_it_points_into():
+    """The plan's structs hold addresses; the tables they name must live as long as the plan."""
+    from zero_amd.inference.decode import DecodePlan, KVCache
+    dec = llama.LlamaForCausalLM(config())
+    cache = KVCache(1, 1, 16, 64, "cpu")
+    cos, sin = torch.zeros(16, 32), torch.zeros(16, 32)
+    plan = DecodePlan(dec, cache, cos, sin)
+    assert plan.structs[0].cos_t == cos.data_ptr() and plan.structs[0].sin_t == sin.data_ptr()
+    alive = [weakref.ref(cos), weakref.ref(sin)]
+    del cos, sin
+    gc.collect()
+    assert all(r() is not None for r in alive)

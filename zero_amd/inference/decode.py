@@ -128,7 +128,7 @@ class DecodePlan:
         # fp32 partials of the split-cache attention (shared by all layers: the stream orders them)
         ws_floats = B * nh * ((cache.max_len + 63) // 64) * (hd + 2)
         self.attn_ws = torch.empty(ws_floats, dtype=torch.float32, device=dev) if USE_SPLIT_ATTENTION else None
-        self.keep = []                                    # views the structs point into
+        self.keep = [cos_t, sin_t]                        # what the structs point into, beside the weights and the cache
         self.structs = []
         for li, layer in enumerate(layers):
             a, m = layer.self_attn, layer.mlp
