@@ -149,3 +149,12 @@ def test_generation_without_an_assistant(stand_ins):
     m = Model(mixed)
     got = paged.generate_paged(m, [prompt(*p) for p in PROMPTS], 5, page_size=2)
     assert got.tolist() == [text(mixed, p, 5) for p in PROMPTS] and len(m.steps) == 5
+
+
+@pytest.mark.parametrize("vocab", [V - 1, V + 1])
+def test_an_assistant_of_another_vocabulary_is_refused(stand_ins, vocab):
+    """Its drafts are looked up in the decoder's embedding table and the decoder's tokens in its own."""
+    m, helper = Model(mixed), Model(mixed, vocab=vocab)
+    with pytest.raises(ValueError, match="vocabular"):
+        paged.generate_paged(m, [prompt(*p) for p in PROMPTS], 6, assistant=helper)
+    assert not m.steps and not helper.steps

@@ -249,6 +249,9 @@ def generate_paged(decoder, prompts: Sequence[torch.Tensor], max_new_tokens: int
     nodes = 1 + draft_width * draft_depth if assistant is not None else 1
     if assistant is not None and (draft_width < 1 or draft_depth < 1):
         raise ValueError("generate: draft_width and draft_depth must be positive")
+    if assistant is not None and assistant.lm_head.weight.shape[0] != decoder.lm_head.weight.shape[0]:
+        raise ValueError(f"generate: vocabularies differ: {assistant.lm_head.weight.shape[0]} tokens of the assistant, "
+                         f"{decoder.lm_head.weight.shape[0]} of the decoder")
     u = None
     if sampling is not None:                             # the numbers that decode.generate draws; drafts past the end: any
         u = torch.rand((max_new_tokens, B), generator=generator, device=device)
