@@ -6,6 +6,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
+from zero_amd.distributed.tensor_parallel import TPContext
 from zero_amd.inference import paged
 
 V, D = 50, 4
@@ -158,3 +159,20 @@ def test_an_assistant_of_another_vocabulary_is_refused(stand_ins, vocab):
     with pytest.raises(ValueError, match="vocabular"):
         paged.generate_paged(m, [prompt(*p) for p in PROMPTS], 6, assistant=helper)
     assert not m.steps and not helper.steps
+
+
+def test_an_assistant_that_is_whole_on_every_rank_runs_whole(stand_ins):
+    """Under tensor parallelism a whole assistant's products are not summed over the ranks, those of a split one are; one
+    that is split over another number of ranks is refused."""
+    group = TPContext(1, 2, reduce_fn=lambda part: part)
+    for world in (1, 2):
+        m, helper = Model(mixed, world=2), Model(mixed, world=world)
+        got = paged.generate_paged(m, [prompt(*PROMPTS[0])], 6, assistant=helper, tp=group)
+        assert got.tolist() == [text(mixed, PROMPTS[0], 6)] and m.steps and helper.steps
+        assert all(tp is group for _, tp in m.steps)
+        for _, tp in helper.steps:
+            assert tp is group if world == 2 else tp.world == 1 and tp.lead and tp.reduce("x") == "x"
+    for tp, world in ((group, 4), (None, 2)):
+        with pytest.raises(ValueError, match="ranks"):
+            paged.generate_paged(Model(mixed, world=tp.world if tp else 1), [prompt(*PROMPTS[0])], 6, tp=tp,
+                                 assistant=Model(mixed, world=world))

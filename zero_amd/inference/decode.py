@@ -240,9 +240,9 @@ def generate(decoder, inputs_embeds: torch.Tensor, attention_mask=None, do_sampl
     Greedy, or with ``do_sample`` by ops.sample's temperature / top_k / top_p / min_p from uniform numbers of ``generator``
     (a device generator; under tensor parallelism every rank passes one of equal seed).  ``attention_mask`` [B, S]: positions
     with 0 are left out, so prompts of different lengths decode as they would alone.  ``assistant``: a decoder of the same
-    vocabulary and width that drafts ``draft_width`` chains of ``draft_depth`` tokens a step; greedy tokens stay those of
-    decoding without it and sampled ones follow the same distributions, up to the rounding of products with other row
-    counts."""
+    vocabulary and width that drafts ``draft_width`` chains of ``draft_depth`` tokens a step (under tensor parallelism split
+    over the same ranks, or whole on every rank); greedy tokens stay those of decoding without it and sampled ones follow the
+    same distributions, up to the rounding of products with other row counts."""
     sampling = dict(temperature=float(temperature), top_k=int(top_k), top_p=float(top_p), min_p=float(min_p)) if do_sample else None
     keep = None if attention_mask is None else attention_mask != 0
     ragged = keep is not None and not bool(keep.all())

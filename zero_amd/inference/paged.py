@@ -209,6 +209,17 @@ def accepted_path(parents: Sequence[int], tokens: Sequence[int], drawn: Sequence
         path.append(nxt[0])
 
 
+def _assistant_tp(assistant, tp: TPContext) -> TPContext:
+    """How the assistant runs beside a decoder of the group ``tp``: split over the same ranks, or whole on each of them (all
+    draft alike: equal weights, equal tokens, kernels that repeat themselves bit for bit)."""
+    layer = assistant.model.layers[0]
+    nh, _, hd, _ = layer.cfg_dims
+    parts = nh * hd // layer.self_attn.q_proj.weight.shape[0]
+    if parts != tp.world and parts != 1:
+        raise ValueError(f"generate: the assistant is split over {parts} ranks, the decoder's group has {tp.world}")
+    return tp if parts == tp.world else TPContext()
+
+
 def _draft(assistant, cache: PagedKVCache, roots: Sequence[Optional[int]], width: int, depth: int, tp) -> List[List[int]]:
     """Tokens of the tree draft_tree(width, depth) under each root (None: a finished sequence, no nodes): the ``width``
     likeliest after the root, then the likeliest after each.  Each level runs the nodes so far again, as the tree of one
@@ -235,7 +246,8 @@ def generate_paged(decoder, prompts: Sequence[torch.Tensor], max_new_tokens: int
                    assistant_prompts: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     """New token ids [B, <= max_new_tokens] (int64) for prompts [S_b, d] of any lengths; sequences that ended are filled
     with ``pad_token_id``.  ``sampling``: ops.sample's settings (None: the largest logit).  ``assistant``: a decoder of the
-    same vocabulary that drafts draft_width chains of draft_depth tokens a step (its prompts default to the decoder's)."""
+    same vocabulary that drafts draft_width chains of draft_depth tokens a step (its prompts default to the decoder's); under
+    tensor parallelism split over the same ranks as the decoder, or whole on every rank."""
     tp = tp or TPContext()
     if not prompts:
         raise ValueError("generate: no prompts")
@@ -252,12 +264,13 @@ def generate_paged(decoder, prompts: Sequence[torch.Tensor], max_new_tokens: int
     if assistant is not None and assistant.lm_head.weight.shape[0] != decoder.lm_head.weight.shape[0]:
         raise ValueError(f"generate: vocabularies differ: {assistant.lm_head.weight.shape[0]} tokens of the assistant, "
                          f"{decoder.lm_head.weight.shape[0]} of the decoder")
+    helper_tp = None if assistant is None else _assistant_tp(assistant, tp)
     u = None
     if sampling is not None:                             # the numbers that decode.generate draws; drafts past the end: any
         u = torch.rand((max_new_tokens, B), generator=generator, device=device)
         u = torch.cat([u, torch.zeros((nodes, B), device=device)])
 
-    def fill(dec, rows):
+    def fill(dec, rows, tp):
         lens = [int(p.shape[0]) for p in rows]
         if min(lens) == 0:
             raise ValueError("generate: an empty prompt")
@@ -277,10 +290,10 @@ def generate_paged(decoder, prompts: Sequence[torch.Tensor], max_new_tokens: int
         us = u[torch.tensor([i for _, i in where]).to(device), torch.tensor([b for b, _ in where]).to(device)]
         return check_drawn(draw_tokens(logits, us, sampling).tolist())
 
-    cache, logits = fill(decoder, prompts)
+    cache, logits = fill(decoder, prompts, tp)
     helper = None
     if assistant is not None:
-        helper, _ = fill(assistant, prompts if assistant_prompts is None else assistant_prompts)
+        helper, _ = fill(assistant, prompts if assistant_prompts is None else assistant_prompts, helper_tp)
     out: List[List[int]] = [[] for _ in range(B)]
     done = [False] * B
 
@@ -297,12 +310,12 @@ def generate_paged(decoder, prompts: Sequence[torch.Tensor], max_new_tokens: int
             tokens = [[] if r is None else [r] for r in roots]
             trees = [[-1] * len(t) for t in tokens]
         else:
-            tokens = _draft(assistant, helper, roots, draft_width, draft_depth, tp)
+            tokens = _draft(assistant, helper, roots, draft_width, draft_depth, helper_tp)
             trees = [draft_tree(draft_width, draft_depth) if t else [] for t in tokens]
             # the assistant's rows of the last level: its step stopped one level short of them
             st = helper.step([len(t) for t in trees], trees)
             forward_paged(assistant, _embed(assistant, [t for ts in tokens for t in ts], device), helper, st,
-                          torch.zeros(1, dtype=torch.int64, device=device), tp)
+                          torch.zeros(1, dtype=torch.int64, device=device), helper_tp)
         step = cache.step([len(t) for t in trees], trees if helper is not None else None)
         logits = forward_paged(decoder, _embed(decoder, [t for ts in tokens for t in ts], device), cache, step, None, tp)
         where = [(b, len(out[b]) + d) for b in range(B) for d in depths(trees[b])]
