@@ -133,6 +133,20 @@ def test_cache_hands_out_pages_and_takes_them_back():
         cache_of(page_size=0)
 
 
+@pytest.mark.parametrize("counts,error", [([8, 4, 8], RuntimeError), ([4, 21, 0], ValueError), ([0, 1, 21], ValueError)],
+                         ids=str)
+def test_a_refused_step_hands_out_nothing(counts, error):
+    """A step that does not fit leaves the pages as they were, those of the sequences before the one that did not fit too."""
+    c = cache_of(n_pages=4)
+    c.step([3, 0, 0])
+    before = (list(c._free), [list(p) for p in c.pages], c.page_table.clone(), list(c.lengths))
+    with pytest.raises(error):
+        c.step(counts)
+    assert (c._free, c.pages, c.lengths) == (before[0], before[1], before[3]) and torch.equal(c.page_table, before[2])
+    c.release(0)
+    c.step([0, 0, 16])                                        # all four pages
+
+
 def test_cache_keeps_a_path_of_a_tree():
     """Rows of the path move to the front, over pages, for all layers; sources that are destinations of others first read."""
     c = cache_of(max_seqs=2, page_size=3)

@@ -95,16 +95,24 @@ class PagedKVCache:
 
     def grow(self, b: int, rows: int):
         """Pages for ``rows`` rows of sequence b."""
-        if rows > self.max_len:
-            raise ValueError(f"KV cache too small: {rows} > {self.max_len}")
-        need = -(-rows // self.page_size) - len(self.pages[b])
-        if need > len(self._free):
-            raise RuntimeError(f"KV cache out of pages: sequence {b} needs {need}, {len(self._free)} are free")
-        for _ in range(need):
-            pg = self._free.pop()
-            self._host_table[b, len(self.pages[b])] = pg
-            self.pages[b].append(pg)
-            self._table = None
+        self._grow_all([(b, rows)])
+
+    def _grow_all(self, wanted):
+        """Pages for (sequence, rows) pairs: for all of them, or, refused, for none."""
+        need = []
+        for b, rows in wanted:
+            if rows > self.max_len:
+                raise ValueError(f"KV cache too small: {rows} > {self.max_len}")
+            need.append(max(-(-rows // self.page_size) - len(self.pages[b]), 0))
+        if sum(need) > len(self._free):
+            raise RuntimeError(f"KV cache out of pages: {sum(need)} needed (of sequences "
+                               f"{[b for (b, _), n in zip(wanted, need) if n]}), {len(self._free)} are free")
+        for (b, _), n in zip(wanted, need):
+            for _ in range(n):
+                pg = self._free.pop()
+                self._host_table[b, len(self.pages[b])] = pg
+                self.pages[b].append(pg)
+                self._table = None
 
     def truncate(self, b: int, rows: int):
         """Sequence b ends at ``rows``; pages past it go back."""
@@ -129,10 +137,10 @@ class PagedKVCache:
         if trees is not None and [len(t) for t in trees] != list(counts):
             raise ValueError("step: trees and counts differ")
         mask = None if trees is None else tree_mask(trees, self.kv.device)       # (refuses what is no tree, before pages go)
+        self._grow_all([(b, self.lengths[b] + n) for b, n in enumerate(counts)])
         positions, slots, ctx, cu = [], [], [], [0]
         for b, n in enumerate(counts):
             base = self.lengths[b]
-            self.grow(b, base + n)
             positions += [base + d for d in (range(n) if trees is None else depths(trees[b]))]
             slots += [self.row(b, base + i) for i in range(n)]
             ctx.append(base + n)
