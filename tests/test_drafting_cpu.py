@@ -176,3 +176,36 @@ def test_an_assistant_that_is_whole_on_every_rank_runs_whole(stand_ins):
         with pytest.raises(ValueError, match="ranks"):
             paged.generate_paged(Model(mixed, world=tp.world if tp else 1), [prompt(*PROMPTS[0])], 6, tp=tp,
                                  assistant=Model(mixed, world=world))
+
+
+def drawing(undrawable):
+    """draw_tokens for sampled rows: the likeliest, or -1 (what ops.sample gives for a row it cannot draw from) where the
+    likeliest token is one of ``undrawable``."""
+    def draw(logits, u, sampling):
+        top = logits.float().argmax(-1)
+        return torch.tensor([-1 if int(t) in undrawable else int(t) for t in top])
+    return draw
+
+
+def test_a_row_without_a_drawable_token_counts_only_where_it_is_taken(stand_ins, monkeypatch):
+    """Rows of drafts that are not accepted, and of what follows the end of a sequence, may hold NaN."""
+    ids, n = PROMPTS[0], 7
+    want = text(mixed, ids, n)
+
+    def wild(tokens):                                        # what follows drafts that are never in the text: 41
+        return 41 if any(t in (30, 33) for t in tokens[len(ids):]) else mixed(tokens)
+    assert not {30, 33, 41} & set(want)
+    monkeypatch.setattr(paged, "draw_tokens", drawing({41}))
+    got = paged.generate_paged(Model(wild), [prompt(*ids)], n, assistant=Model(lambda t: 30), draft_width=2, draft_depth=1,
+                               sampling=dict(temperature=1.0))
+    assert got.tolist() == [want]
+    eos = want[2]                                            # a full draft goes on behind the end token
+    monkeypatch.setattr(paged, "draw_tokens", drawing({want[3]}))
+    got = paged.generate_paged(Model(mixed), [prompt(*ids)], n, assistant=Model(mixed), draft_width=1, draft_depth=4,
+                               sampling=dict(temperature=1.0), eos_token_id=eos)
+    assert got.tolist() == [want[:3]]
+    for helper in (None, Model(mixed)):                      # and is refused in the text itself, the first token among it
+        for bad in (want[0], want[3]):
+            monkeypatch.setattr(paged, "draw_tokens", drawing({bad}))
+            with pytest.raises(FloatingPointError):
+                paged.generate_paged(Model(mixed), [prompt(*ids)], n, assistant=helper, sampling=dict(temperature=1.0))

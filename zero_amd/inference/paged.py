@@ -296,7 +296,7 @@ def generate_paged(decoder, prompts: Sequence[torch.Tensor], max_new_tokens: int
         if sampling is None:
             return draw_tokens(logits, None, None).tolist()
         us = u[torch.tensor([i for _, i in where]).to(device), torch.tensor([b for b, _ in where]).to(device)]
-        return check_drawn(draw_tokens(logits, us, sampling).tolist())
+        return draw_tokens(logits, us, sampling).tolist()
 
     cache, logits = fill(decoder, prompts, tp)
     helper = None
@@ -305,9 +305,9 @@ def generate_paged(decoder, prompts: Sequence[torch.Tensor], max_new_tokens: int
     out: List[List[int]] = [[] for _ in range(B)]
     done = [False] * B
 
-    def emit(b, token):
+    def emit(b, token):                                  # (a row that is not taken may have nothing to draw from)
         if not done[b]:
-            out[b].append(token)
+            out[b].append(check_drawn([token])[0])
             done[b] = token in eos or len(out[b]) >= max_new_tokens
 
     for b, t in enumerate(draw(logits, [(b, 0) for b in range(B)])):
