@@ -239,6 +239,8 @@ int zk_llama_decode_mlp(const zk_decode_layer_t* L, const void* xa, void* out, i
  * page_size >= 1; row r of sequence b is row r % page_size of page page_table[b][r / page_size].
  * Indices in device memory are checked in the kernels against the sizes given here: a slot or a page number out of
  * range is passed over, nothing outside the arrays is touched.
+ * A launch has fewer than 2^32 threads, so an append takes fewer than 2^24 tokens, and attention fewer than 2^24
+ * workgroups (by kv heads, sequences and shares of max_ctx; -22 beyond, from zk_attn_paged_ws too).
  *
  * zk_kv_append_paged: T new tokens, packed rows q|k|v (row stride ldqkv, left untouched).  Token t is turned by row
  * positions[t] of the cos / sin tables ([table_rows][rot_dim / 2] fp32, the values zk_rope takes) over the first
@@ -284,6 +286,7 @@ int zk_attn_paged_ws(int64_t B, int64_t T, int64_t max_q, int64_t max_ctx, int64
  * call.  For the call: temperature in [0, 2^20], top_k >= 0, top_p in (0, 1], min_p in [0, 1], else -22.  Per row:
  * temperature <= 0 or NaN takes the first token and values above 2^20 act as 2^20; top_k <= 0, top_p >= 1 or NaN and
  * min_p <= 0 or NaN keep everything; top_p <= 0 or min_p > 1 keeps the first token.
+ * Fewer than 2^22 rows a call (a launch has fewer than 2^32 threads).
  * -inf logits are never drawn; a row of nothing else gives -1 with logprob -inf, a row with a NaN -1 with NaN.
  * (tf generate(do_sample=True) with its logits processors; the reference itself decodes greedily, ref:vlm_infer.py:267.) */
 int zk_sample(const void* logits, const float* u, const float* temperature_rows, const int32_t* top_k_rows,

@@ -74,6 +74,26 @@ def test_sample_refusals(bad):
     assert sample(**bad) == EINVAL
 
 
+@pytest.mark.parametrize("call,good,bad", [
+    (append, dict(T=0), dict(T=1 << 24)),                                             # a token a workgroup of 256 threads
+    (sample, dict(rows=0), dict(rows=1 << 22)),                                       # a row a workgroup of 1024
+    (attn, dict(T=0), dict(T=4096, B=4096, max_q=1, max_ctx=1 << 18, Hq=32, Hkv=8, ldq=4096, ldo=4096)),     # shares
+    (attn, dict(T=0), dict(T=65536, B=65536, max_q=1, max_ctx=8200, Hq=64, Hkv=4, ldq=8192, ldo=8192)),      # merge
+    (attn, dict(T=0), dict(T=1 << 23, B=4, max_q=1 << 22, max_ctx=1 << 22, Hq=128, Hkv=1, ldq=16384, ldo=16384)),
+], ids=["append", "sample", "attention-shares", "attention-merge", "attention-tiles"])
+def test_calls_of_more_threads_than_a_launch_has_are_refused_before_it(call, good, bad):
+    """2^32 threads and more are no launch."""
+    assert call(**good) == OK and call(**bad) == EINVAL
+
+
+def test_attention_workspace_of_a_call_that_cannot_be_launched():
+    from zero_amd import ops
+    from zero_amd._lib import ZeroHipError
+    with pytest.raises(ZeroHipError):
+        ops.attn_paged_ws_floats(4096, 4096, 1, 1 << 18, 32, 8, 128)
+    assert ops.attn_paged_ws_floats(4096, 4096, 1, 1 << 17, 32, 8, 128) > 0
+
+
 def test_wrappers_refuse_host_tensors():
     from zero_amd import ops
     b = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731

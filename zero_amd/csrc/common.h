@@ -27,6 +27,9 @@ typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
     if (e__ != hipSuccess) return ZK_ELAUNCH;               \
   } while (0)
 
+// a launch has fewer than 2^32 threads in x
+inline bool zk_too_many(int64_t workgroups, int64_t threads) { return workgroups * threads > 0xFFFFFFFFLL; }
+
 // compile-time loop: f(std::integral_constant<int, 0>{}) ... f(std::integral_constant<int, N - 1>{})
 template <class F, int... Is>
 __device__ __forceinline__ void static_for_impl(F&& f, std::integer_sequence<int, Is...>) {

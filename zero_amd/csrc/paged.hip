@@ -995,6 +995,7 @@ extern "C" int zk_kv_append_paged(const void* qkv, const float* cos_t, const flo
                                   int64_t Hkv, int64_t head_dim, int64_t rot_dim, int64_t table_rows, int64_t ldqkv,
                                   int64_t ldq, int64_t cache_rows, int interleaved, hipStream_t stream) {
   if (T < 0 || T > 0x7FFFFFFF || Hq <= 0 || Hkv <= 0 || Hq % Hkv || (head_dim != 64 && head_dim != 128)) return ZK_EINVAL;
+  if (zk_too_many(T, 256)) return ZK_EINVAL;
   if ((Hq + 2 * Hkv) * head_dim > (1 << 24)) return ZK_EINVAL;
   if (rot_dim < 16 || (rot_dim & 15) || rot_dim > head_dim || table_rows <= 0 || table_rows > 0x7FFFFFFF) return ZK_EINVAL;
   if (cache_rows <= 0 || cache_rows > 0x7FFFFFFF || (ldqkv & 7) || (ldq & 7)) return ZK_EINVAL;
@@ -1015,7 +1016,10 @@ extern "C" int zk_attn_paged_ws(int64_t B, int64_t T, int64_t max_q, int64_t max
   if (!ws_floats || B <= 0 || T < 0 || max_q <= 0 || max_ctx <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv) return ZK_EINVAL;
   if ((head_dim != 64 && head_dim != 128) || T >= kMaxRows || max_q > 0x7FFFFFFF || max_ctx > 0x7FFFFF00) return ZK_EINVAL;
   if (B >= kMaxRows || Hq > (1 << 17) || B * Hkv > (1 << 28) || T * Hq > 0x7FFFFFFF) return ZK_EINVAL;
-  *ws_floats = T ? plan_of(B, T, max_q, max_ctx, Hq, Hkv, head_dim).ws : 0;
+  const Plan p = T ? plan_of(B, T, max_q, max_ctx, Hq, Hkv, head_dim) : Plan{};
+  if (zk_too_many(p.grid, p.waves == 8 ? 512 : 256)) return ZK_EINVAL;
+  if (p.splits > 16 && zk_too_many(T * Hq * (head_dim / 32), kMergeThreads)) return ZK_EINVAL;
+  *ws_floats = p.ws;
   return ZK_OK;
 }
 
@@ -1038,7 +1042,6 @@ extern "C" int zk_attn_paged(const void* q, const void* k_cache, const void* v_c
     return ZK_EINVAL;
   if (T == 0) return ZK_OK;
   const Plan p = plan_of(B, T, max_q, max_ctx, Hq, Hkv, head_dim);
-  if (p.grid > 0x7FFFFFF0 || (p.mt != 8 && p.splits > 16 && T * Hq * (head_dim / 32) > 0x7FFFFFF0)) return ZK_EINVAL;
   int lg = 0;                                       // page_mul: the 31-bit reciprocal, rounded up (exact below 2^31)
   while ((int64_t)1 << lg < page_size) ++lg;
   const unsigned mul = (unsigned)((((unsigned long long)1 << (31 + lg)) / (unsigned long long)page_size) + 1);

@@ -480,6 +480,7 @@ extern "C" int zk_sample(const void* logits, const float* u, const float* temper
                          float min_p, int64_t* tokens, float* logprobs, int64_t rows, int64_t V, int64_t ld,
                          hipStream_t stream) {
   if (rows < 0 || rows > 0x7FFFFFFF || V <= 0 || V > 0x7FFFFFFF || ld < V) return ZK_EINVAL;
+  if (zk_too_many(rows, kThreads)) return ZK_EINVAL;
   if (!logits || !u || !tokens || !logprobs || (reinterpret_cast<uintptr_t>(logits) & 1)) return ZK_EINVAL;
   // settings of the whole call: a number is asked for (NaN is not), top_p and min_p are shares
   if (!temperature_rows && !(temperature >= 0.f && temperature <= kMaxTemperature)) return ZK_EINVAL;
