@@ -100,7 +100,7 @@ struct PagedArgs {
   float *part_o, *part_ml;
   int* shares;
   int T, B, max_q, Hq, Hkv, page_size, n_pages, table_cols, ld_table, mask_words;
-  int tiles, splits, split_keys, groups;
+  int splits, split_keys;
   unsigned page_mul, page_shift;   // key / page_size = key * page_mul >> page_shift for every key < 2^31
   long long ldq, ldo;
   float scale;
@@ -165,23 +165,6 @@ __device__ __forceinline__ int cache_row(const PagedArgs& a, int b, int key, int
   const unsigned pg = (unsigned)a.table[(size_t)b * a.ld_table + at];
   return pg < (unsigned)a.n_pages ? (int)(pg * (unsigned)a.page_size + ((unsigned)key - at * (unsigned)a.page_size)) : -1;
 }
-
-// workgroup -> (sequence, share, kv head, row tile).  Row tiles of one (sequence, share, kv head) read the same keys: they
-// are neighbours on one XCD (workgroups of equal id % 8), so that its L2 serves all but the first; these groups are dealt to
-// the XCDs in turn, so that long sequences load all of them.
-struct Work {
-  int tile, split, kvh, b;
-  bool any;                                         // false: an id past the last group, from rounding up to whole eights
-  __device__ __forceinline__ Work(const PagedArgs& a) {
-    int w = (int)(blockIdx.x >> 3);
-    tile = w % a.tiles;
-    w = w / a.tiles * 8 + (int)(blockIdx.x & 7);
-    any = w < a.groups;
-    kvh = w % a.Hkv; w /= a.Hkv;
-    split = w % a.splits;
-    b = w / a.splits;
-  }
-};
 
 // Shares of the tile kernel's work, from the lengths themselves (the host knows bounds only; shares cut by the largest
 // length left half of the CUs idle on a ragged batch).  A share is `q` 64-key tiles of one (sequence, kv head, 128-row
@@ -263,8 +246,9 @@ __device__ __forceinline__ bool not_finite(unsigned w) {
 }
 
 // =========================================================================================
-// attention.  The q rows of a group of Hq / Hkv heads read the same keys, so a tile is 16 * MT rows (token i, head g of the
-// group at row i * G + g) of one kv head, and a workgroup is (sequence, kv head, row tile, share of the keys).
+// attention of few rows.  The q rows of a group of Hq / Hkv heads read the same keys, so a workgroup takes all rows of one kv
+// head (token i, head g of the group at row i * G + g; 16 * MT at most) over one share of a sequence's keys.  Workgroup ids
+// run over sequences, shares, kv heads: neighbours are on different XCDs, so that a long sequence loads all of them.
 // Its W waves take 32-key pieces in turn, each with a softmax of its own (running maximum and sum in fp32, no barrier in
 // the loop), merged through LDS at the end; shares of one sequence are merged by attn_paged_merge_kernel.
 // Products: 16x16x32 MFMAs.  S^T[key][row] = K Q^T, K fragments straight from memory to registers (16 rows x 64 bytes per
@@ -284,13 +268,11 @@ __global__ __launch_bounds__(64 * W, W == 4 && MT == 1 && HD == 64 ? 4 : 2) void
   __shared__ float sm[W][16 * MT], sl[W][16 * MT];
   const int tid = threadIdx.x, lane = tid & 63, g4 = lane >> 4, col = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Work w(a);
-  if (!w.any) return;
-  const int kvh = w.kvh, tile = w.tile, split = w.split, b = w.b;
+  const int kvh = (int)blockIdx.x % a.Hkv, split = (int)blockIdx.x / a.Hkv % a.splits, b = (int)blockIdx.x / a.Hkv / a.splits;
   const Seq s(a, b);
-  const int G = a.Hq / a.Hkv, rows = s.rows, r0 = tile * 16 * MT, kvw = a.Hkv * HD;
+  const int G = a.Hq / a.Hkv, rows = s.rows, kvw = a.Hkv * HD;
   const int ks = split * a.split_keys;
-  if (r0 >= rows || (split > 0 && ks >= s.len)) return;
+  if (!rows || (split > 0 && ks >= s.len)) return;
   const int ke = split == a.splits - 1 ? s.len : min(s.len, ks + a.split_keys);
   const bool alone = ks == 0 && ke == s.len;        // no other share of this sequence
   const float sc = a.scale * kLog2e;
@@ -301,7 +283,7 @@ __global__ __launch_bounds__(64 * W, W == 4 && MT == 1 && HD == 64 ? 4 : 2) void
   int tok[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    const int r = r0 + mt * 16 + col;
+    const int r = mt * 16 + col;
     tok[mt] = min(r, rows - 1) / G;
     const bf16_t* qp = a.q + (size_t)(s.q0 + tok[mt]) * a.ldq + (size_t)(kvh * G + min(r, rows - 1) % G) * HD + 8 * g4;
 #pragma unroll
@@ -387,8 +369,8 @@ __global__ __launch_bounds__(64 * W, W == 4 && MT == 1 && HD == 64 ? 4 : 2) void
     }
   };
 
-  // pieces that every row of the tile sees whole: up to the tile's first token in a chain, to the new tokens in a tree
-  const int bulk = min(ke, s.first + (a.mask ? 0 : r0 / G + 1));
+  // pieces that every row sees whole: up to the first new token in a chain, to the new tokens in a tree
+  const int bulk = min(ke, s.first + (a.mask ? 0 : 1));
   int base = ks + 32 * wave;
   if (base + 32 <= bulk) {
     int row = cache_row(a, b, base + (lane & 31), bulk);
@@ -439,7 +421,7 @@ __global__ __launch_bounds__(64 * W, W == 4 && MT == 1 && HD == 64 ? 4 : 2) void
     if (!__any(odd)) {
       product();
     } else {
-      // infinities or NaN among rows that some of the tile may not see: key by key, rows with p = 0 passed over
+      // infinities or NaN among cache rows that some tokens may not see: key by key, rows with p = 0 passed over
 #pragma unroll 1
       for (int vrow = 0; vrow < 32; ++vrow) {
 #pragma unroll
@@ -488,13 +470,12 @@ __global__ __launch_bounds__(64 * W, W == 4 && MT == 1 && HD == 64 ? 4 : 2) void
       for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4*>(xo + (wave * 16 + col) * LDO + d * 16 + 4 * g4) = o[mt][d] * f;
     }
     __syncthreads();
-    const int r = r0 + mt * 16 + orow;
+    const int r = mt * 16 + orow;
     if (r < rows) {
-      const int lr = mt * 16 + orow;
-      const float M = top(lr);
+      const float M = top(r);
       float L = 0.f, y[per];
 #pragma unroll
-      for (int w = 0; w < W; ++w) L += M == -INFINITY ? 0.f : sl[w][lr] * fast_exp2(sm[w][lr] - M);
+      for (int w = 0; w < W; ++w) L += M == -INFINITY ? 0.f : sl[w][r] * fast_exp2(sm[w][r] - M);
 #pragma unroll
       for (int e = 0; e < per; ++e) {
         y[e] = 0.f;
@@ -941,7 +922,7 @@ __global__ __launch_bounds__(256) void attn_paged_merge_tiles_kernel(PagedArgs a
 
 // shape of a launch: host arithmetic on the sizes alone
 struct Plan {
-  int mt, waves, tiles, splits, split_keys;         // mt: 16-row groups of the stream kernel's tile, 8 = the tile kernel
+  int mt, waves, splits, split_keys;                // mt: 16-row groups of the stream kernel, 8 = the tile kernel
   int64_t grid, header, parts, ws;                  // workgroups; floats of the header, parts, floats altogether
 };
 inline Plan plan_of(int64_t B, int64_t T, int64_t max_q, int64_t max_ctx, int64_t Hq, int64_t Hkv, int64_t hd) {
@@ -950,9 +931,8 @@ inline Plan plan_of(int64_t B, int64_t T, int64_t max_q, int64_t max_ctx, int64_
   // 20 rows of width 128 over 2 x 8192 (16 x 1024) keys: 23.2 (18.2) us by two 16-row groups, 24.7 (20.7) by tiles; over
   // 8 x 4096: 39.0, 36.6.  24 rows of width 64 over 8 x 4096: 41.5 by two groups, 39.0 by tiles.  4 rows: 18 against 24.
   p.mt = rows <= 16 ? 1 : rows <= 32 && hd == 128 ? 2 : 8;
-  p.tiles = (int)((rows + 16 * p.mt - 1) / (16 * p.mt));
-  const int64_t groups = B * Hkv * p.tiles;
   if (p.mt == 8) {
+    const int64_t groups = B * Hkv * ((rows + 127) / 128);
     // shares are cut on the device; no sequence of up to four 64-key tiles is, nor any where there is work for two rounds
     const int64_t slots = hd == 64 ? kTileSlots<64> : kTileSlots<128>;
     const bool shared = max_ctx > 256 && T * Hq < 128 * 2 * slots;
@@ -964,6 +944,7 @@ inline Plan plan_of(int64_t B, int64_t T, int64_t max_q, int64_t max_ctx, int64_
     // shares of the keys: as many as fill the 512 workgroups that the CUs hold at two each, none under 128 keys (a piece
     // for each wave) and none over 512: the lengths of a batch differ, and small shares even that out (48 sequences of
     // 700 to 8192: 150 us with 1024 keys, 140 with 512)
+    const int64_t groups = B * Hkv;
     int64_t keys = (max_ctx * groups + 511) / 512;
     keys = (keys + 127) / 128 * 128;
     keys = keys < 128 ? 128 : keys > 512 ? 512 : keys;
@@ -979,7 +960,7 @@ inline Plan plan_of(int64_t B, int64_t T, int64_t max_q, int64_t max_ctx, int64_
     }
     p.split_keys = (int)keys;
     p.splits = (int)((max_ctx + keys - 1) / keys);
-    p.grid = (B * Hkv * p.splits + 7) / 8 * 8 * p.tiles;
+    p.grid = groups * p.splits;
     p.parts = p.splits > 1 ? T * Hq * p.splits : 0;
   }
   p.ws = p.header + p.parts * (hd + 2);
@@ -1049,7 +1030,7 @@ extern "C" int zk_attn_paged(const void* q, const void* k_cache, const void* v_c
   PagedArgs a{(const bf16_t*)q, (const bf16_t*)k_cache, (const bf16_t*)v_cache, (bf16_t*)out, page_table, ctx_lens, cu_q,
               (const unsigned long long*)tree_mask, part_o, part_o ? part_o + p.parts * head_dim : nullptr, (int*)ws, (int)T,
               (int)B, (int)max_q, (int)Hq, (int)Hkv, (int)page_size, (int)n_pages, (int)table_cols, (int)ld_table,
-              (int)mask_words, p.tiles, p.splits, p.split_keys, (int)(B * Hkv * p.splits), mul, (unsigned)(31 + lg),
+              (int)mask_words, p.splits, p.split_keys, mul, (unsigned)(31 + lg),
               (long long)ldq, (long long)ldo, scale};
   const bool one_page = page_size % 64 == 0;
   void (*kern)(PagedArgs) =
