@@ -265,8 +265,11 @@ int zk_kv_append_paged(const void* qkv, const float* cos_t, const float* sin_t, 
  * not see may hold anything, NaN included.  max_q >= every n_b (tokens past it are not computed) and max_ctx (an
  * upper bound of ctx_lens that only shapes the launch) come from the host, so a captured graph serves growing caches.
  * ws: at least what zk_attn_paged_ws says (fp32, 16-byte aligned, null when 0); calls that may overlap need one each.
- * head_dim 64 or 128, any Hq / Hkv; scale > 0; sequences of up to 2^30 rows; softmax in fp32, probabilities rounded to
- * bf16 for the product with the values (tf:llama:182-205, eager_attention_forward with a mask). */
+ * head_dim 64 or 128, any Hq / Hkv; scale > 0; sequences of up to 2^30 rows.  Scores, maxima, exponentials and sums are
+ * fp32; probabilities are rounded to bf16 for the product with the values, and with more than 16 rows a kv head (max_q
+ * times Hq / Hkv; 32 at head_dim 128) the sum that divides them takes the rounded ones too, so that neither side leans.
+ * Repeated calls agree bit for bit; a sequence's last bits depend on the batch around it, which cuts its keys into shares.
+ * (tf:llama:182-205, eager_attention_forward with a mask.) */
 int zk_attn_paged(const void* q, const void* k_cache, const void* v_cache, void* out, const int32_t* page_table,
                   const int32_t* ctx_lens, const int32_t* cu_q, const int64_t* tree_mask, float* ws, int64_t ws_floats,
                   int64_t T, int64_t B, int64_t max_q, int64_t max_ctx, int64_t Hq, int64_t Hkv, int64_t head_dim,

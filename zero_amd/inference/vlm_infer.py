@@ -1,6 +1,6 @@
 """Zero-shot grafting inference (ref:inference/vlm_infer.py:191-277) from token ids on: encoder +
 adapter prefix (``Zero._forward``, the same function as on the training path), splice into the prompt
-at the image token, pad, greedy ``generate`` on the FULL decoder (``enable_translator=False``,
+at the image token, pad, ``generate`` (greedy unless asked to sample) on the FULL decoder (``enable_translator=False``,
 ref:vlm_infer.py:57) — on one GPU or tensor parallel (distributed/tensor_parallel.py).
 The tokenizer / chat template and the image file preprocessing stay outside (no tokenizer offline,
 SURVEY.md §8c): callers pass pixel tensors and id lists that contain ``img_id`` once."""

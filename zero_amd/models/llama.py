@@ -196,7 +196,8 @@ class LlamaForCausalLM(nn.Module):
 
     def generate(self, inputs_embeds=None, attention_mask=None, do_sample=False, max_new_tokens=20,
                  use_cache=True, **kwargs):
-        """Greedy decoding with a KV cache (ref:inference/vlm_infer.py:259-270); new token ids only."""
+        """Decoding with a KV cache, greedy unless ``do_sample`` (ref:inference/vlm_infer.py:259-270); new token ids only;
+        further arguments: inference.decode.generate."""
         from ..inference.decode import generate
         return generate(self, inputs_embeds, attention_mask=attention_mask, do_sample=do_sample,
                         max_new_tokens=max_new_tokens, use_cache=use_cache, **kwargs)
