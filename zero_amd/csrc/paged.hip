@@ -514,7 +514,9 @@ __global__ __launch_bounds__(64 * W, W == 4 && MT == 1 && HD == 64 ? 4 : 2) void
 // chunk-swizzled, two stages, one barrier per tile; S^T = K Q^T and O^T += V^T P^T in 32x32x16 MFMAs with the row on
 // the lane, as in zk_attn_fwd.  Each wave's instructions bind, matrix and vector in turn: a 64-key tile takes a workgroup
 // 2.5 us, of which 1.7 us stay without the matrix instructions and 2.0 us without the DMA.  2048 new tokens over 32768 rows
-// (32 heads over 8 of 128, 1.06 TFLOP): 1046 to 1129 us from card to card, 940 to 1010 TFLOP/s.  Short
+// (32 heads over 8 of 128, 1.06 TFLOP; 512 workgroups, one round): calls of 1046 to 1129 us from card to card, 940 to 1010
+// TFLOP/s, and 1100 to 1177 us a launch in a kernel trace of nine.  2112 to 2560 tokens take 1800 us, a second round that is
+// nearly empty; a whole prompt's row tiles differ in length: 2048 tokens 76 us, 8192 659 (452 and 835 TFLOP/s).  Short
 // chunks are latency: a share's start, its stores and the merge cost as much as four of its tiles.
 // =========================================================================================
 // LDS-DMA of 16 bytes a lane to consecutive LDS from the wave-uniform `dst` on; sources per lane, or a uniform base and a
