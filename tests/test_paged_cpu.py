@@ -79,8 +79,9 @@ def test_sample_refusals(bad):
     (sample, dict(rows=0), dict(rows=1 << 22)),                                       # a row a workgroup of 1024
     (attn, dict(T=0), dict(T=4096, B=4096, max_q=1, max_ctx=1 << 18, Hq=32, Hkv=8, ldq=4096, ldo=4096)),     # shares
     (attn, dict(T=0), dict(T=65536, B=65536, max_q=1, max_ctx=8200, Hq=64, Hkv=4, ldq=8192, ldo=8192)),      # merge
+    (attn, dict(T=0), dict(T=1 << 22, B=1 << 22, max_q=1, max_ctx=1536, Hq=16, Hkv=1, ldq=2048, ldo=2048)),  # of few shares
     (attn, dict(T=0), dict(T=1 << 23, B=4, max_q=1 << 22, max_ctx=1 << 22, Hq=128, Hkv=1, ldq=16384, ldo=16384)),
-], ids=["append", "sample", "attention-shares", "attention-merge", "attention-tiles"])
+], ids=["append", "sample", "attention-shares", "attention-merge", "attention-merge-few", "attention-tiles"])
 def test_calls_of_more_threads_than_a_launch_has_are_refused_before_it(call, good, bad):
     """2^32 threads and more are no launch."""
     assert call(**good) == OK and call(**bad) == EINVAL

@@ -924,8 +924,8 @@ __global__ __launch_bounds__(256) void attn_paged_merge_tiles_kernel(PagedArgs a
 
 // shape of a launch: host arithmetic on the sizes alone
 struct Plan {
-  int mt, waves, splits, split_keys;                // mt: 16-row groups of the stream kernel, 8 = the tile kernel
-  int64_t grid, header, parts, ws;                  // workgroups; floats of the header, parts, floats altogether
+  int mt, waves, splits, split_keys, merge_heads;   // mt: 16-row groups of the stream kernel, 8 = the tile kernel
+  int64_t grid, merge, header, parts, ws;           // workgroups of both launches; floats of the header, parts, floats altogether
 };
 inline Plan plan_of(int64_t B, int64_t T, int64_t max_q, int64_t max_ctx, int64_t Hq, int64_t Hkv, int64_t hd) {
   Plan p{};
@@ -942,6 +942,10 @@ inline Plan plan_of(int64_t B, int64_t T, int64_t max_q, int64_t max_ctx, int64_
     p.grid = shared && groups < 2 * slots ? 2 * slots : groups;
     p.header = shared ? (B + 64) / 64 * 64 : 0;
     p.parts = shared ? 2 * slots * 128 : 0;
+    // a wave a row while every row's wave is resident at once (256 CUs x 32): 160 rows x 8 heads of 50 shares 33.2 -> 31.4 us
+    // a call, 89 x 2 x 8 31.3 -> 28.6; beyond, two rows a wave: 1000 x 16 48.6, 51.3 by one
+    p.merge_heads = T * Hq <= 8192 ? 1 : 2;
+    p.merge = shared ? T * ((Hq + 4 * p.merge_heads - 1) / (4 * p.merge_heads)) : 0;
   } else {
     // shares of the keys: as many as fill the 512 workgroups that the CUs hold at two each, none under 128 keys (a piece
     // for each wave) and none over 512: the lengths of a batch differ, and small shares even that out (48 sequences of
@@ -964,6 +968,9 @@ inline Plan plan_of(int64_t B, int64_t T, int64_t max_q, int64_t max_ctx, int64_
     p.splits = (int)((max_ctx + keys - 1) / keys);
     p.grid = groups * p.splits;
     p.parts = p.splits > 1 ? T * Hq * p.splits : 0;
+    // few shares: a wave a row (7 shares of 32 rows 8.2 us a call, 8.8 by workgroups; 4 of 1536 rows 83.7, 90.9; but 64 of
+    // 32 rows 21.1, 18.4, and 32 of 128 rows 48.2, 47.0)
+    p.merge = p.splits == 1 ? 0 : p.splits <= 16 ? (T * Hq + 3) / 4 : T * Hq * (hd / 32);
   }
   p.ws = p.header + p.parts * (hd + 2);
   return p;
@@ -1000,8 +1007,7 @@ extern "C" int zk_attn_paged_ws(int64_t B, int64_t T, int64_t max_q, int64_t max
   if ((head_dim != 64 && head_dim != 128) || T >= kMaxRows || max_q > 0x7FFFFFFF || max_ctx > 0x7FFFFF00) return ZK_EINVAL;
   if (B >= kMaxRows || Hq > (1 << 17) || B * Hkv > (1 << 28) || T * Hq > 0x7FFFFFFF) return ZK_EINVAL;
   const Plan p = T ? plan_of(B, T, max_q, max_ctx, Hq, Hkv, head_dim) : Plan{};
-  if (zk_too_many(p.grid, p.waves == 8 ? 512 : 256)) return ZK_EINVAL;
-  if (p.splits > 16 && zk_too_many(T * Hq * (head_dim / 32), kMergeThreads)) return ZK_EINVAL;
+  if (zk_too_many(p.grid, p.waves == 8 ? 512 : 256) || zk_too_many(p.merge, kMergeThreads)) return ZK_EINVAL;
   *ws_floats = p.ws;
   return ZK_OK;
 }
@@ -1039,22 +1045,14 @@ extern "C" int zk_attn_paged(const void* q, const void* k_cache, const void* v_c
       head_dim == 128 ? (p.mt == 1 ? (p.waves == 4 ? attn_paged_stream_kernel<128, 1, 4> : attn_paged_stream_kernel<128, 1, 8>) : p.mt == 2 ? attn_paged_stream_kernel<128, 2, 4> : one_page ? attn_paged_tile_kernel<128, true> : attn_paged_tile_kernel<128, false>)
                       : (p.mt == 1 ? (p.waves == 4 ? attn_paged_stream_kernel<64, 1, 4> : attn_paged_stream_kernel<64, 1, 8>) : one_page ? attn_paged_tile_kernel<64, true> : attn_paged_tile_kernel<64, false>);
   hipLaunchKernelGGL(kern, dim3((unsigned)p.grid), dim3(p.waves == 8 ? 512 : 256), 0, stream, a);
-  if (p.splits > 1 && p.mt == 8) {
-    // a wave a row while every row's wave is resident at once (256 CUs x 32): 160 rows x 8 heads of 50 shares 33.2 -> 31.4 us
-    // a call, 89 x 2 x 8 31.3 -> 28.6; beyond, two rows a wave: 1000 x 16 48.6, 51.3 by one
-    const bool one = T * Hq <= 8192;
-    void (*merge)(PagedArgs) = head_dim == 128 ? (one ? attn_paged_merge_tiles_kernel<128, 1> : attn_paged_merge_tiles_kernel<128, 2>)
-                                               : (one ? attn_paged_merge_tiles_kernel<64, 1> : attn_paged_merge_tiles_kernel<64, 2>);
-    const int64_t heads = one ? 4 : 8;
-    hipLaunchKernelGGL(merge, dim3((unsigned)(T * ((Hq + heads - 1) / heads))), dim3(256), 0, stream, a);
-  } else if (p.splits > 1) {
-    // few shares: a wave a row (7 shares of 32 rows 8.2 us a call, 8.8 by workgroups; 4 of 1536 rows 83.7, 90.9; but 64 of
-    // 32 rows 21.1, 18.4, and 32 of 128 rows 48.2, 47.0)
-    const bool few = p.splits <= 16;
-    void (*merge)(PagedArgs) = head_dim == 128 ? (few ? attn_paged_merge_few_kernel<128> : attn_paged_merge_kernel<128>)
-                                               : (few ? attn_paged_merge_few_kernel<64> : attn_paged_merge_kernel<64>);
-    const int64_t wgs = few ? (T * Hq + 3) / 4 : T * Hq * (head_dim / 32);
-    hipLaunchKernelGGL(merge, dim3((unsigned)wgs), dim3(kMergeThreads), 0, stream, a);
+  if (p.splits > 1) {
+    const bool one = p.merge_heads == 1, few = p.splits <= 16;
+    void (*merge)(PagedArgs) =
+        p.mt == 8 ? (head_dim == 128 ? (one ? attn_paged_merge_tiles_kernel<128, 1> : attn_paged_merge_tiles_kernel<128, 2>)
+                                     : (one ? attn_paged_merge_tiles_kernel<64, 1> : attn_paged_merge_tiles_kernel<64, 2>))
+                  : (head_dim == 128 ? (few ? attn_paged_merge_few_kernel<128> : attn_paged_merge_kernel<128>)
+                                     : (few ? attn_paged_merge_few_kernel<64> : attn_paged_merge_kernel<64>));
+    hipLaunchKernelGGL(merge, dim3((unsigned)p.merge), dim3(kMergeThreads), 0, stream, a);
   }
   ZK_CHECK_LAUNCH();
   return ZK_OK;
