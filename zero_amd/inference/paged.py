@@ -16,7 +16,6 @@ from typing import List, Optional, Sequence
 import numpy as np
 import torch
 
-from .. import functional as ZF
 from .. import ops
 from ..distributed.tensor_parallel import TPContext
 from .decode import BF16, check_drawn, draw_tokens, eos_ids, mlp_infer, qkv_infer
